@@ -20,13 +20,16 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "liba2a.so")
 
 A2A_OK, A2A_ERR_CONFIG, A2A_ERR_CAPACITY, A2A_ERR_TIMEOUT, A2A_ERR_STATE, A2A_ERR_ROUTING = range(6)
-DTYPE_BF16, DTYPE_FP16 = 0, 1
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
 PAYLOAD = {"direct": 0, "dedup": 1, "fp8": 2}
 SCHEDULE = {"phased": 0, "pipelined": 1}
 COMBINE = {"pull": 0, "push": 1}
 GROUP_PHASE = {"pipe_send": 0, "pipe_expert": 1, "pipe_combine": 2, "send": 3, "recv": 4, "expert": 5, "recv_expert": 6,
                "combine": 7}
+ACTIVATION = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "swiglu": 4}
+SCORE = {"softmax": 0, "sigmoid": 1}
 MAX_WORLD, MAX_EXPERTS, MAX_TOPK = 8, 1024, 32
+MAX_PRODUCT, MAX_LAYER_TOKENS = 65536, 256
 
 
 class Config(C.Structure):
@@ -44,6 +47,30 @@ class Call(C.Structure):
     """One rank's tensors in a call on a whole group."""
     _fields_ = [("x", C.c_void_p), ("topk_idx", C.c_void_p), ("topk_weights", C.c_void_p), ("y", C.c_void_p),
                 ("num_tokens", C.c_int32)]
+
+
+class Gate(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("stride", C.c_int64), ("bias", C.c_void_p), ("indices", C.c_void_p),
+                ("weights", C.c_void_p)] + [(n, C.c_int32) for n in (
+                    "tokens", "experts", "topk", "dtype", "score", "renormalize")] + [("scale", C.c_float)]
+
+
+class Linear(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "weight", "bias", "residual", "y")]
+                + [(n, C.c_int64) for n in ("x_stride", "weight_stride", "residual_stride", "y_stride")]
+                + [(n, C.c_int32) for n in ("tokens", "inputs", "outputs", "dtype", "out_dtype", "bias_dtype", "activation")])
+
+
+class Layer(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "topk_idx", "topk_weights", "gate_up", "down", "residual", "y", "workspace")]
+                + [("workspace_bytes", C.c_size_t)]
+                + [(n, C.c_int32) for n in ("tokens", "topk", "experts", "hidden_dim", "inner", "dtype")])
+
+
+class Experts(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("rows", "counts", "gate_up", "down", "out", "workspace")]
+                + [("workspace_bytes", C.c_size_t)]
+                + [(n, C.c_int32) for n in ("local_experts", "world", "capacity", "hidden_dim", "inner", "dtype")])
 
 
 class A2AError(RuntimeError):
@@ -87,6 +114,13 @@ SIGNATURES = {
     "a2a_copy_route": (_I, [_VP, _VP, _VP, _VP]),
     "a2a_route_noalloc": (_I, [_VP, _I, _I, _I, _VP, _VP, _VP]),
     "a2a_histogram256": (_I, [_VP, C.c_size_t, _VP, _VP]),
+    "a2a_gate": (_I, [C.POINTER(Gate), _VP]),
+    "a2a_linear": (_I, [C.POINTER(Linear), _VP]),
+    "a2a_layer_workspace": (C.c_size_t, [_I, _I, _I, _I]),
+    "a2a_layer": (_I, [C.POINTER(Layer), _VP]),
+    "a2a_experts_workspace": (C.c_size_t, [_I, _I, _I, _I]),
+    "a2a_experts": (_I, [C.POINTER(Experts), _VP]),
+    "a2a_product_status": (_I, [C.POINTER(C.c_int32)]),
     "a2a_status": (_I, [_VP, C.POINTER(Status)]),
     "a2a_status_clear": (_I, [_VP]),
     "a2a_status_peek": (_I, [_VP]),

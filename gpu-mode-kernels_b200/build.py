@@ -12,16 +12,22 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "liba2a.so")
-SOURCES = [os.path.join(CSRC, "a2a.cu"), os.path.join(CSRC, "a2a_noalloc.cu"), os.path.join(CSRC, "histogram.cu")]
+SOURCES = [os.path.join(CSRC, "a2a.cu"), os.path.join(CSRC, "a2a_noalloc.cu"), os.path.join(CSRC, "histogram.cu"),
+           os.path.join(CSRC, "gate.cu"), os.path.join(CSRC, "product.cu")]
 HEADERS = [os.path.join(CSRC, "a2a_kernels.cuh"), os.path.join(CSRC, "a2a_pipe.cuh"), os.path.join(CSRC, "a2a_near.cuh"),
            os.path.join(CSRC, "a2a_solo.cuh"),
            os.path.join(CSRC, "a2a_device.cuh"),
+           os.path.join(CSRC, "product_device.cuh"), os.path.join(CSRC, "product_rows.cuh"), os.path.join(CSRC, "product_tiles.cuh"),
            os.path.join(ROOT, "include", "a2a.h")]
+FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
+         "-I", os.path.join(ROOT, "include"), "-I", CSRC]
+OBJ_DIR = os.path.join(PKG_DIR, "build")
 HOST_SOURCE = os.path.join(CSRC, "host.cpp")
 
 
@@ -74,15 +80,18 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Compile both if one is missing or older than the sources; return the library's path."""
     if not force and not needs_build():
         return LIB_PATH
-    cmd = [
-        nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-        "-shared", "-Xcompiler", "-fPIC", "-cudart", "static",
-        "-I", os.path.join(ROOT, "include"), "-I", CSRC,
-        "-o", LIB_PATH, *SOURCES,
-    ]
-    if verbose:
-        cmd[1:1] = ["-Xptxas", "-v"]
-    run("nvcc", cmd, verbose)
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    newest_header = max(os.path.getmtime(f) for f in HEADERS + [os.path.abspath(__file__)])
+
+    def compile_one(source: str) -> str:
+        target = os.path.join(OBJ_DIR, os.path.basename(source) + ".o")
+        if force or not os.path.exists(target) or os.path.getmtime(target) < max(newest_header, os.path.getmtime(source)):
+            run("nvcc", [nvcc_path(), *(["-Xptxas", "-v"] if verbose else []), *FLAGS, "-c", "-o", target, source], verbose)
+        return target
+
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        objects = list(pool.map(compile_one, SOURCES))
+    run("nvcc", [nvcc_path(), *FLAGS, "-shared", "-cudart", "static", "-o", LIB_PATH, *objects], verbose)
     build_host(verbose)
     return LIB_PATH
 

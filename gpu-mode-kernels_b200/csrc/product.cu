@@ -1,0 +1,293 @@
+// The experts of a layer and the dense products beside them: argument checks, tensor maps and launches.
+//
+// Up to 16 rows of a dense product and up to eight tokens of a layer go through product_rows.cuh (loads, mma.sync: nothing
+// counts but reading the weights), more through product_tiles.cuh (tcgen05).
+#include <atomic>
+
+#include "product_device.cuh"
+#include "product_rows.cuh"
+#include "product_tiles.cuh"
+
+namespace {
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                CUtensorMapFloatOOBfill);
+
+// The driver's encoder of tensor maps, looked up through the runtime, so that the library needs no driver to be loaded.
+EncodeTiled encoder() {
+    static std::atomic<void*> found{nullptr};
+    void* fn = found.load(std::memory_order_acquire);
+    if (fn == nullptr) {
+        cudaDriverEntryPointQueryResult how;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &how) != cudaSuccess ||
+            how != cudaDriverEntryPointSuccess)
+            return nullptr;
+        found.store(fn, std::memory_order_release);
+    }
+    return reinterpret_cast<EncodeTiled>(fn);
+}
+
+CUtensorMapDataType map_type(int dtype) {
+    return dtype == A2A_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// Rows [rows][inner], `stride` elements apart, in boxes of `box` rows by 64.
+int rows_map(CUtensorMap* map, int dtype, const void* p, long long rows, int inner, long long stride, int box) {
+    const EncodeTiled encode = encoder();
+    if (encode == nullptr) return -(int)cudaErrorNotSupported;
+    const cuuint64_t sizes[2] = {(cuuint64_t)inner, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t boxes[2] = {kTileInner, (cuuint32_t)box}, ones[2] = {1, 1};
+    return encode(map, map_type(dtype), 2, const_cast<void*>(p), sizes, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? A2A_OK
+               : A2A_ERR_CONFIG;
+}
+
+// Weights [groups][features], or [groups][gate, up][features], rows of `inner` values `stride` apart, in boxes of 128 rows by 64; with
+// gate and up a box steps from one to the other first.
+int weights_map(CUtensorMap* map, int dtype, const void* p, int groups, int features, bool paired, int inner, long long stride) {
+    const EncodeTiled encode = encoder();
+    if (encode == nullptr) return -(int)cudaErrorNotSupported;
+    const cuuint64_t row = (cuuint64_t)stride * 2, halves = paired ? 2 : 1;
+    const cuuint64_t sizes[4] = {(cuuint64_t)inner, halves, (cuuint64_t)features, (cuuint64_t)groups};
+    const cuuint64_t strides[3] = {paired ? row * features : row, row, row * features * halves};
+    const cuuint32_t boxes[4] = {kTileInner, (cuuint32_t)halves, (cuuint32_t)(kTileRows / halves), 1}, ones[4] = {1, 1, 1, 1};
+    return encode(map, map_type(dtype), 4, const_cast<void*>(p), sizes, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? A2A_OK
+               : A2A_ERR_CONFIG;
+}
+
+int sm_count(int* sms) {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return -(int)e;
+    int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+        if ((e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return -(int)e;
+        if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    }
+    *sms = n;
+    return A2A_OK;
+}
+
+// A launch that may get ready while the one before it in the stream ends; its kernel waits for that one itself.
+int launch_after(const void* fn, int grid, int threads, size_t shared, void* params, cudaStream_t st) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t launch{};
+    launch.gridDim = dim3(grid);
+    launch.blockDim = dim3(threads);
+    launch.dynamicSmemBytes = shared;
+    launch.stream = st;
+    launch.attrs = &attr;
+    launch.numAttrs = 1;
+    void* args[] = {params};
+    const cudaError_t e = cudaLaunchKernelExC(&launch, fn, args);
+    return e == cudaSuccess ? A2A_OK : -(int)e;
+}
+
+template <TilesOp kOp, typename T>
+int launch_tiles(const TilesParams& p, int grid, cudaStream_t st) {
+    const void* fn = reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T>);
+    static std::atomic<unsigned long long> opted{0};  // a bit a device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return -(int)e;
+    if (dev >= 64 || !(opted.load(std::memory_order_acquire) >> dev & 1)) {
+        if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTilesSharedBytes)) != cudaSuccess) return -(int)e;
+        if (dev < 64) opted.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    return launch_after(fn, grid, kTilesThreads, kTilesSharedBytes, const_cast<TilesParams*>(&p), st);
+}
+
+template <RowsOp kOp, typename T, int kWide>
+int launch_rows(const RowsParams& p, int grid, cudaStream_t st) {
+    return launch_after(reinterpret_cast<const void*>(&product_rows_kernel<kOp, T, kWide>), grid, kRowsThreads, 0, const_cast<RowsParams*>(&p), st);
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <typename T>
+int linear_of(const a2a_linear_args& a, int sms, cudaStream_t st) {
+    const bool paired = a.activation == A2A_ACT_SWIGLU;
+    if (a.tokens <= 2 * kRowsTokens) {
+        RowsParams p{};
+        p.weights = a.weight, p.weights_stride = a.weight_stride;
+        p.x = a.x, p.x_stride = a.x_stride;
+        p.inner = a.inputs, p.features = a.outputs, p.tokens = a.tokens;
+        p.activation = a.activation, p.paired = paired, p.out_fp32 = a.out_dtype == A2A_DTYPE_FP32, p.bias_fp32 = a.bias_dtype == A2A_DTYPE_FP32;
+        p.bias = a.bias, p.residual = a.residual, p.residual_stride = a.residual_stride, p.y = a.y, p.y_stride = a.y_stride;
+        const int grid = a.outputs < sms ? a.outputs : sms;
+        return a.tokens <= kRowsTokens ? launch_rows<kRowsDense, T, 1>(p, grid, st) : launch_rows<kRowsDense, T, 2>(p, grid, st);
+    }
+    TilesParams p{};
+    p.inner = a.inputs, p.features = a.outputs, p.paired = paired, p.groups = 1, p.tokens = a.tokens;
+    p.activation = a.activation, p.out_fp32 = a.out_dtype == A2A_DTYPE_FP32, p.bias_fp32 = a.bias_dtype == A2A_DTYPE_FP32;
+    p.bias = a.bias, p.residual = a.residual, p.residual_stride = a.residual_stride, p.y = a.y, p.y_stride = a.y_stride;
+    p.columns = a.tokens < kMaxColumns ? (a.tokens + 15) / 16 * 16 : kMaxColumns;
+    int rc = weights_map(&p.weights, a.dtype, a.weight, 1, a.outputs, paired, a.inputs, a.weight_stride);
+    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.inputs, a.x_stride, p.columns);
+    if (rc != A2A_OK) return rc;
+    const int height = paired ? kTileRows / 2 : kTileRows;
+    const long long tiles = (long long)((a.outputs + height - 1) / height) * ((a.tokens + p.columns - 1) / p.columns);
+    return launch_tiles<kDense, T>(p, (int)(tiles < sms ? tiles : sms), st);
+}
+
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// The workspace of a layer: the experts' inner values, and for more than a few tokens the rows of every pair and the tickets.
+struct LayerSpace {
+    size_t hidden, parts, tickets, end;
+};
+LayerSpace layer_space(int tokens, int topk, int hidden_dim, int inner) {
+    LayerSpace s{};
+    const size_t pairs = (size_t)tokens * topk;
+    s.parts = round256(pairs * inner * 2);
+    if (tokens <= kRowsTokens) {
+        s.tickets = s.end = s.parts;
+    } else {
+        s.tickets = s.parts + round256(pairs * hidden_dim * 4);
+        s.end = s.tickets + round256((size_t)tokens * ((hidden_dim + kTileRows - 1) / kTileRows) * 4);
+    }
+    return s;
+}
+
+bool sizes_fit(int experts, int hidden_dim, int inner) {
+    return experts >= 1 && experts <= A2A_MAX_EXPERTS && hidden_dim >= 8 && hidden_dim % 8 == 0 && hidden_dim <= A2A_MAX_PRODUCT && inner >= 8 &&
+           inner % 8 == 0 && inner <= A2A_MAX_PRODUCT;
+}
+
+template <typename T>
+int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
+    uint8_t* const space = static_cast<uint8_t*>(a.workspace);
+    const LayerSpace at = layer_space(a.tokens, a.topk, a.hidden_dim, a.inner);
+    if (a.tokens <= kRowsTokens) {
+        RowsParams p{};
+        p.weights = a.gate_up, p.weights_stride = a.hidden_dim;
+        p.x = a.x, p.x_stride = a.hidden_dim;
+        p.inner = a.hidden_dim, p.features = a.inner, p.tokens = a.tokens;
+        p.y = space, p.y_stride = a.inner;
+        p.indices = a.topk_idx, p.weights_of = a.topk_weights, p.topk = a.topk, p.experts = a.experts;
+        const int rc = launch_rows<kRowsUp, T, 1>(p, sms, st);
+        if (rc != A2A_OK) return rc;
+        p.weights = a.down, p.weights_stride = a.inner;
+        p.x = space, p.x_stride = a.inner;
+        p.inner = a.inner, p.features = a.hidden_dim;
+        p.residual = a.residual, p.residual_stride = a.hidden_dim;
+        p.y = a.y, p.y_stride = a.hidden_dim;
+        return launch_rows<kRowsDown, T, 1>(p, a.hidden_dim < sms ? a.hidden_dim : sms, st);
+    }
+    TilesParams p{};
+    p.groups = a.experts, p.tokens = a.tokens, p.topk = a.topk, p.indices = a.topk_idx, p.weights_of = a.topk_weights;
+    p.hidden = space, p.parts = reinterpret_cast<float*>(space + at.parts), p.tickets = reinterpret_cast<int*>(space + at.tickets);
+    p.ticket_count = a.tokens * ((a.hidden_dim + kTileRows - 1) / kTileRows);
+    p.columns = kMaxColumns;
+    p.inner = a.hidden_dim, p.features = a.inner, p.paired = 1;
+    int rc = weights_map(&p.weights, a.dtype, a.gate_up, a.experts, a.inner, true, a.hidden_dim, a.hidden_dim);
+    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.hidden_dim, a.hidden_dim, 1);
+    if (rc == A2A_OK) rc = launch_tiles<kLayerUp, T>(p, sms, st);
+    if (rc != A2A_OK) return rc;
+    p.inner = a.inner, p.features = a.hidden_dim, p.paired = 0;
+    p.residual = a.residual, p.y = a.y;
+    rc = weights_map(&p.weights, a.dtype, a.down, a.experts, a.hidden_dim, false, a.inner, a.inner);
+    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, p.hidden, (long long)a.tokens * a.topk, a.inner, a.inner, 1);
+    return rc == A2A_OK ? launch_tiles<kLayerDown, T>(p, sms, st) : rc;
+}
+
+template <typename T>
+int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {
+    const long long rows = (long long)a.local_experts * a.world * a.capacity;
+    TilesParams p{};
+    p.groups = a.local_experts, p.counts = a.counts, p.world = a.world, p.capacity = a.capacity, p.hidden = a.workspace;
+    p.columns = kMaxColumns;
+    p.inner = a.hidden_dim, p.features = a.inner, p.paired = 1;
+    int rc = weights_map(&p.weights, a.dtype, a.gate_up, a.local_experts, a.inner, true, a.hidden_dim, a.hidden_dim);
+    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.rows, rows, a.hidden_dim, a.hidden_dim, 1);
+    if (rc == A2A_OK) rc = launch_tiles<kSlabUp, T>(p, sms, st);
+    if (rc != A2A_OK) return rc;
+    p.inner = a.inner, p.features = a.hidden_dim, p.paired = 0, p.y = a.out;
+    rc = weights_map(&p.weights, a.dtype, a.down, a.local_experts, a.hidden_dim, false, a.inner, a.inner);
+    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.workspace, rows, a.inner, a.inner, 1);
+    return rc == A2A_OK ? launch_tiles<kSlabDown, T>(p, sms, st) : rc;
+}
+
+bool dtype16(int dtype) { return dtype == A2A_DTYPE_BF16 || dtype == A2A_DTYPE_FP16; }
+
+}  // namespace
+
+extern "C" int a2a_linear(const a2a_linear_args* args, void* stream) {
+    if (args == nullptr) return A2A_ERR_CONFIG;
+    const a2a_linear_args& a = *args;
+    if (!dtype16(a.dtype) || (a.out_dtype != a.dtype && a.out_dtype != A2A_DTYPE_FP32)) return A2A_ERR_CONFIG;
+    if (a.bias != nullptr && a.bias_dtype != a.dtype && a.bias_dtype != A2A_DTYPE_FP32) return A2A_ERR_CONFIG;
+    if (a.activation < A2A_ACT_NONE || a.activation > A2A_ACT_SWIGLU) return A2A_ERR_CONFIG;
+    if (a.tokens < 0 || a.outputs < 1 || a.outputs > A2A_MAX_PRODUCT || a.inputs < 8 || a.inputs % 8 != 0 || a.inputs > A2A_MAX_PRODUCT)
+        return A2A_ERR_CONFIG;
+    if (a.tokens == 0) return A2A_OK;
+    if (a.x == nullptr || a.weight == nullptr || a.y == nullptr || !aligned(a.x) || !aligned(a.weight)) return A2A_ERR_CONFIG;
+    if (a.x_stride < a.inputs || a.x_stride % 8 != 0 || a.weight_stride < a.inputs || a.weight_stride % 8 != 0) return A2A_ERR_CONFIG;
+    if (a.y_stride < a.outputs || (a.residual != nullptr && a.residual_stride < 0)) return A2A_ERR_CONFIG;
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc != A2A_OK) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return a.dtype == A2A_DTYPE_BF16 ? linear_of<__nv_bfloat16>(a, sms, st) : linear_of<__half>(a, sms, st);
+}
+
+extern "C" size_t a2a_layer_workspace(int num_tokens, int experts_per_token, int hidden_dim, int inner) {
+    if (num_tokens < 0 || experts_per_token < 1 || hidden_dim < 1 || inner < 1) return 0;
+    return layer_space(num_tokens, experts_per_token, hidden_dim, inner).end;
+}
+
+extern "C" int a2a_layer(const a2a_layer_args* args, void* stream) {
+    if (args == nullptr) return A2A_ERR_CONFIG;
+    const a2a_layer_args& a = *args;
+    if (!dtype16(a.dtype) || !sizes_fit(a.experts, a.hidden_dim, a.inner)) return A2A_ERR_CONFIG;
+    if (a.tokens < 0 || a.tokens > A2A_MAX_LAYER_TOKENS || a.topk < 1 || a.topk > A2A_MAX_TOPK) return A2A_ERR_CONFIG;
+    if (a.tokens == 0) return A2A_OK;
+    if (a.x == nullptr || a.topk_idx == nullptr || a.topk_weights == nullptr || a.gate_up == nullptr || a.down == nullptr || a.y == nullptr ||
+        a.workspace == nullptr)
+        return A2A_ERR_CONFIG;
+    if (!aligned(a.x) || !aligned(a.gate_up) || !aligned(a.down) || reinterpret_cast<uintptr_t>(a.workspace) % 256 != 0) return A2A_ERR_CONFIG;
+    if (a.workspace_bytes < layer_space(a.tokens, a.topk, a.hidden_dim, a.inner).end) return A2A_ERR_CAPACITY;
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc != A2A_OK) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return a.dtype == A2A_DTYPE_BF16 ? layer_of<__nv_bfloat16>(a, sms, st) : layer_of<__half>(a, sms, st);
+}
+
+extern "C" size_t a2a_experts_workspace(int local_experts, int world_size, int capacity, int inner) {
+    if (local_experts < 1 || world_size < 1 || capacity < 1 || inner < 1) return 0;
+    return round256((size_t)local_experts * world_size * capacity * inner * 2);
+}
+
+extern "C" int a2a_experts(const a2a_experts_args* args, void* stream) {
+    if (args == nullptr) return A2A_ERR_CONFIG;
+    const a2a_experts_args& a = *args;
+    if (!dtype16(a.dtype) || !sizes_fit(a.local_experts, a.hidden_dim, a.inner)) return A2A_ERR_CONFIG;
+    if (a.world < 1 || a.world > A2A_MAX_WORLD || a.capacity < 1 || a.capacity > 65535) return A2A_ERR_CONFIG;
+    if (a.rows == nullptr || a.counts == nullptr || a.gate_up == nullptr || a.down == nullptr || a.out == nullptr || a.workspace == nullptr)
+        return A2A_ERR_CONFIG;
+    if (!aligned(a.rows) || !aligned(a.gate_up) || !aligned(a.down) || reinterpret_cast<uintptr_t>(a.workspace) % 256 != 0) return A2A_ERR_CONFIG;
+    if (a.workspace_bytes < a2a_experts_workspace(a.local_experts, a.world, a.capacity, a.inner)) return A2A_ERR_CAPACITY;
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc != A2A_OK) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return a.dtype == A2A_DTYPE_BF16 ? experts_of<__nv_bfloat16>(a, sms, st) : experts_of<__half>(a, sms, st);
+}
+
+extern "C" int a2a_product_status(int32_t* code) {
+    if (code == nullptr) return A2A_ERR_CONFIG;
+    cudaError_t e = cudaDeviceSynchronize();
+    int zero = 0, got = 0;
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&got, g_product_error, sizeof(int));
+    if (e == cudaSuccess && got != 0) e = cudaMemcpyToSymbol(g_product_error, &zero, sizeof(int));
+    *code = got;
+    return e == cudaSuccess ? A2A_OK : -(int)e;
+}

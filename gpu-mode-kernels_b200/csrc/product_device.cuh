@@ -1,0 +1,192 @@
+// What the kernels of the products share: element types, the epilogue's arithmetic, barriers with bounded waits, the
+// tensor copies and the tensor core's instructions as inline PTX.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+#include <stdint.h>
+
+#include "a2a.h"
+
+namespace {
+
+// A wait inside a kernel ends after this long whatever happens: every barrier here is completed by the same block (or its
+// cluster), so one that is not is a fault of this code, and it is to end in an error instead of a GPU that does not answer.
+constexpr long long kWaitNs = 2000000000ll;
+
+// Set by a kernel whose wait ran out; read and cleared by a2a_product_status.
+__device__ int g_product_error;
+
+__device__ __forceinline__ long long now_ns() {
+    long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+// ---- element types -----------------------------------------------------------------------------
+template <typename T>
+struct Element;
+template <>
+struct Element<__nv_bfloat16> {
+    static constexpr unsigned kFormat = 1;  // of the tensor core's instruction descriptor
+    static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+};
+template <>
+struct Element<__half> {
+    static constexpr unsigned kFormat = 0;
+    static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+};
+
+// A value of `T` or of fp32, by a flag that is the same for a whole launch.
+template <typename T>
+__device__ __forceinline__ float load_any(const void* p, size_t i, bool fp32) {
+    return fp32 ? static_cast<const float*>(p)[i] : Element<T>::to_float(static_cast<const T*>(p)[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store_any(void* p, size_t i, float v, bool fp32) {
+    if (fp32)
+        static_cast<float*>(p)[i] = v;
+    else
+        static_cast<T*>(p)[i] = Element<T>::from_float(v);
+}
+
+// ---- the epilogue's arithmetic: fp32, on the fp32 sums of a product -------------------------------
+__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
+
+__device__ __forceinline__ float activate(float v, int activation) {
+    switch (activation) {
+        // relu passes a NaN on, as torch's does
+        case A2A_ACT_RELU: return v < 0.0f ? 0.0f : v;
+        case A2A_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+        case A2A_ACT_SILU: return silu(v);
+        default: return v;
+    }
+}
+
+// ---- barriers in shared memory -------------------------------------------------------------------
+__device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void barrier_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_addr(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_init_done() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void barrier_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(shared_addr(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+// Waits for the phase of `parity`; false where the block has given up, or does now because the time has run out.
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+    if (barrier_try(bar, parity)) return true;
+    const long long begin = now_ns();
+    for (;;) {
+        for (int i = 0; i < 64; ++i)
+            if (barrier_try(bar, parity)) return true;
+        if (*gave_up) return false;
+        if (now_ns() - begin > kWaitNs) {
+            *gave_up = 1;
+            return false;
+        }
+    }
+}
+
+// ---- tensor copies, global -> this block's shared memory -------------------------------------------
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+__device__ __forceinline__ void copy_tile_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(shared_addr(dst)), "l"(map), "r"(shared_addr(bar)), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_tile_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(shared_addr(dst)), "l"(map), "r"(shared_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+// Four rows anywhere in the matrix, one under the other.
+__device__ __forceinline__ void copy_rows_4(void* dst, const CUtensorMap* map, int x, int r0, int r1, int r2, int r3, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(shared_addr(dst)), "l"(map), "r"(shared_addr(bar)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+        : "memory");
+}
+
+// ---- tensor core (tcgen05) -------------------------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(where)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+}
+__device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tcgen05_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void tcgen05_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t descriptor, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(descriptor), "r"((uint32_t)add)
+        : "memory");
+}
+// 16 columns of this warp's 32 lanes: a lane's values of columns c to c + 15.
+__device__ __forceinline__ void tmem_load_16(uint32_t tmem, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(tmem));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// A K-major operand in shared memory, rows of 128 bytes in the 128-byte swizzle: groups of eight rows are 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand_descriptor(const void* p) {
+    return (uint64_t)((shared_addr(p) & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+// fp32 sums of products of `format` (Element::kFormat), 128 rows by `columns`, both operands K-major.
+__device__ __forceinline__ uint32_t instruction_descriptor(unsigned format, int columns) {
+    return 1u << 4 | format << 7 | format << 10 | (uint32_t)(columns >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+}
+
+// Whether all of `threads` threads, which meet here, say yes.
+__device__ __forceinline__ bool named_all(int id, int threads, bool yes) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %3, 0;\n\t"
+        "barrier.cta.red.and.pred p, %1, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all)
+        : "r"(id), "r"(threads), "r"((uint32_t)yes)
+        : "memory");
+    return all != 0;
+}
+__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+}  // namespace

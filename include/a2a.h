@@ -346,6 +346,83 @@ int64_t a2a_launch_count(a2a_ctx* ctx);
 /* Bytes of the symmetric region / of the local scratch of this context. */
 size_t a2a_symmetric_bytes(a2a_ctx* ctx);
 
+/* ---- The layer around the all-to-all: gate, experts, dense products -----------------------------------
+ * No counterpart in the reference, whose experts are a placeholder (reference.py:262) and whose routing is drawn at random
+ * (reference.py:33-43).  None of these calls needs a context; they run on the current device, allocate nothing, keep nothing from
+ * one call for the next and never synchronise; workspaces are the caller's, 256-byte aligned, of the size the *_workspace function
+ * gives, and not shared by calls that may run at the same time.  Element types are A2A_DTYPE_BF16 and
+ * A2A_DTYPE_FP16; sums are fp32.  Values too large for fp16 become infinite, in an expert's inner values too. */
+enum { A2A_DTYPE_FP32 = 2 };
+enum { A2A_ACT_NONE = 0, A2A_ACT_RELU = 1, A2A_ACT_GELU = 2, A2A_ACT_SILU = 3, A2A_ACT_SWIGLU = 4 };
+enum { A2A_SCORE_SOFTMAX = 0, A2A_SCORE_SIGMOID = 1 };
+/* longest row of a matrix and most rows of one (twice that with SwiGLU); most tokens of a2a_layer */
+enum { A2A_MAX_PRODUCT = 65536, A2A_MAX_LAYER_TOKENS = 256 };
+
+/* Gate: indices and weights [tokens, topk] from logits [tokens, experts] (rows `stride` apart), as a2a_route and a2a_forward take
+ * them.  score s = softmax or sigmoid of the logits; chosen are the topk largest logits, or, with a bias [experts], the largest s + bias
+ * (in 64 bits), in descending order, ties to the lowest index; a NaN ranks above everything.  weight = scale * s, divided by the sum of the
+ * chosen s if renormalize is not zero (0 where that sum is 0, as for a row of nothing but -inf with softmax).  -inf excludes an
+ * expert as long as topk others are there. */
+typedef struct a2a_gate_args {
+    const void* logits; /* dtype: any of the three */
+    int64_t stride;
+    const float* bias;  /* or NULL */
+    int32_t* indices;
+    float* weights;
+    int32_t tokens, experts, topk, dtype, score, renormalize;
+    float scale;
+} a2a_gate_args;
+int a2a_gate(const a2a_gate_args* args, void* stream);
+
+/* Dense product y = act(x weight^T + bias) + residual: x [tokens, inputs], weight [outputs, inputs] (A2A_ACT_SWIGLU: [2 outputs,
+ * inputs], gate rows before up rows, act = silu(gate) * up, bias [2 outputs]), y and residual [tokens, outputs] of out_dtype (dtype or fp32),
+ * bias of dtype or fp32.  Strides in elements; inputs, x_stride and weight_stride multiples of 8, x and weight 16-byte aligned. y overlaps
+ * no input but residual, which it may be. */
+typedef struct a2a_linear_args {
+    const void *x, *weight, *bias, *residual;
+    void* y;
+    int64_t x_stride, weight_stride, residual_stride, y_stride;
+    int32_t tokens, inputs, outputs, dtype, out_dtype, bias_dtype, activation;
+} a2a_linear_args;
+int a2a_linear(const a2a_linear_args* args, void* stream);
+
+/* A whole layer of a few tokens (at most A2A_MAX_LAYER_TOKENS) on one GPU, in two launches: y[t] = residual[t] + sum over k of w[t, k] *
+ * down_e (silu(gate_e x[t]) * up_e x[t]), e = topk_idx[t, k]; gate_up [experts, 2 inner, hidden_dim] (gate rows before up rows),
+ * down [experts, hidden_dim, inner], all contiguous.  An index outside 0..experts-1 marks no expert; the same expert twice counts twice.
+ * y overlaps no input but residual, which it may be. */
+typedef struct a2a_layer_args {
+    const void* x;
+    const int32_t* topk_idx;
+    const float* topk_weights;
+    const void *gate_up, *down, *residual;
+    void* y;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t tokens, topk, experts, hidden_dim, inner, dtype;
+} a2a_layer_args;
+size_t a2a_layer_workspace(int num_tokens, int experts_per_token, int hidden_dim, int inner);
+int a2a_layer(const a2a_layer_args* args, void* stream);
+
+/* The experts on the rows that a dispatch has left: rows [local_experts, world, capacity, hidden_dim] and counts [world, 4, local_experts] as
+ * a2a_expert_buffers gives them (entry 0 of the four is read; a count outside 0..capacity is taken for the nearest of the two).  out has the
+ * shape of rows and is either rows itself or does not overlap them; what lies behind a slab's count is left as it is.  Between
+ * a2a_dispatch_recv and a2a_expert_done it is the real expert op of that hook. */
+typedef struct a2a_experts_args {
+    const void* rows;
+    const int32_t* counts;
+    const void *gate_up, *down;
+    void* out;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t local_experts, world, capacity, hidden_dim, inner, dtype;
+} a2a_experts_args;
+size_t a2a_experts_workspace(int local_experts, int world_size, int capacity, int inner);
+int a2a_experts(const a2a_experts_args* args, void* stream);
+
+/* What the products on the current device recorded since the last call: A2A_OK, or A2A_ERR_TIMEOUT where a wait inside a kernel ran out
+ * (its outputs are not valid).  Synchronises the device. */
+int a2a_product_status(int32_t* code);
+
 #ifdef __cplusplus
 }
 #endif
