@@ -23,7 +23,7 @@ SOURCES = [os.path.join(CSRC, "a2a.cu"), os.path.join(CSRC, "a2a_noalloc.cu"), o
 HEADERS = [os.path.join(CSRC, "a2a_kernels.cuh"), os.path.join(CSRC, "a2a_pipe.cuh"), os.path.join(CSRC, "a2a_near.cuh"),
            os.path.join(CSRC, "a2a_solo.cuh"),
            os.path.join(CSRC, "a2a_device.cuh"),
-           os.path.join(CSRC, "product_device.cuh"), os.path.join(CSRC, "product_rows.cuh"), os.path.join(CSRC, "product_tiles.cuh"),
+           os.path.join(CSRC, "product_device.cuh"), os.path.join(CSRC, "product_tiles.cuh"),
            os.path.join(ROOT, "include", "a2a.h")]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
          "-I", os.path.join(ROOT, "include"), "-I", CSRC]

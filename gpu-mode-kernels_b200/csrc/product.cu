@@ -1,11 +1,10 @@
 // The experts of a layer and the dense products beside them: argument checks, tensor maps and launches.
 //
-// Up to 16 rows of a dense product and up to eight tokens of a layer go through product_rows.cuh (loads, mma.sync: nothing
-// counts but reading the weights), more through product_tiles.cuh (tcgen05).
+// All of them are product_tiles.cuh's kernel.
+#include <algorithm>
 #include <atomic>
 
 #include "product_device.cuh"
-#include "product_rows.cuh"
 #include "product_tiles.cuh"
 
 namespace {
@@ -44,15 +43,15 @@ int rows_map(CUtensorMap* map, int dtype, const void* p, long long rows, int inn
                : A2A_ERR_CONFIG;
 }
 
-// Weights [groups][features], or [groups][gate, up][features], rows of `inner` values `stride` apart, in boxes of 128 rows by 64; with
-// gate and up a box steps from one to the other first.
-int weights_map(CUtensorMap* map, int dtype, const void* p, int groups, int features, bool paired, int inner, long long stride) {
+// Weights [groups][features], or [groups][gate, up][features], rows of `inner` values `stride` apart, in boxes of `box` features by 64;
+// with gate and up a box steps from one to the other first.
+int weights_map(CUtensorMap* map, int dtype, const void* p, int groups, int features, bool paired, int inner, long long stride, int box) {
     const EncodeTiled encode = encoder();
     if (encode == nullptr) return -(int)cudaErrorNotSupported;
     const cuuint64_t row = (cuuint64_t)stride * 2, halves = paired ? 2 : 1;
     const cuuint64_t sizes[4] = {(cuuint64_t)inner, halves, (cuuint64_t)features, (cuuint64_t)groups};
     const cuuint64_t strides[3] = {paired ? row * features : row, row, row * features * halves};
-    const cuuint32_t boxes[4] = {kTileInner, (cuuint32_t)halves, (cuuint32_t)(kTileRows / halves), 1}, ones[4] = {1, 1, 1, 1};
+    const cuuint32_t boxes[4] = {kTileInner, (cuuint32_t)halves, (cuuint32_t)box, 1}, ones[4] = {1, 1, 1, 1};
     return encode(map, map_type(dtype), 4, const_cast<void*>(p), sizes, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? A2A_OK
@@ -73,40 +72,89 @@ int sm_count(int* sms) {
     return A2A_OK;
 }
 
-// A launch that may get ready while the one before it in the stream ends; its kernel waits for that one itself.
-int launch_after(const void* fn, int grid, int threads, size_t shared, void* params, cudaStream_t st) {
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t launch{};
-    launch.gridDim = dim3(grid);
-    launch.blockDim = dim3(threads);
-    launch.dynamicSmemBytes = shared;
-    launch.stream = st;
-    launch.attrs = &attr;
-    launch.numAttrs = 1;
-    void* args[] = {params};
-    const cudaError_t e = cudaLaunchKernelExC(&launch, fn, args);
-    return e == cudaSuccess ? A2A_OK : -(int)e;
-}
-
+// Lets the kernel have its shared memory on the current device.
 template <TilesOp kOp, typename T>
-int launch_tiles(const TilesParams& p, int grid, cudaStream_t st) {
-    const void* fn = reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T>);
+int opt_in() {
     static std::atomic<unsigned long long> opted{0};  // a bit a device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return -(int)e;
-    if (dev >= 64 || !(opted.load(std::memory_order_acquire) >> dev & 1)) {
-        if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTilesSharedBytes)) != cudaSuccess) return -(int)e;
-        if (dev < 64) opted.fetch_or(1ull << dev, std::memory_order_release);
-    }
-    return launch_after(fn, grid, kTilesThreads, kTilesSharedBytes, const_cast<TilesParams*>(&p), st);
+    if (dev < 64 && (opted.load(std::memory_order_acquire) >> dev & 1)) return A2A_OK;
+    e = cudaFuncSetAttribute((const void*)&product_tiles_kernel<kOp, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTilesSharedBytes);
+    if (e != cudaSuccess) return -(int)e;
+    if (dev < 64) opted.fetch_or(1ull << dev, std::memory_order_release);
+    return A2A_OK;
 }
 
-template <RowsOp kOp, typename T, int kWide>
-int launch_rows(const RowsParams& p, int grid, cudaStream_t st) {
-    return launch_after(reinterpret_cast<const void*>(&product_rows_kernel<kOp, T, kWide>), grid, kRowsThreads, 0, const_cast<RowsParams*>(&p), st);
+// A launch that may get ready while the one before it in the stream ends (its kernel waits for that one itself), in clusters of `cluster` blocks.
+template <TilesOp kOp, typename T>
+int launch_tiles(const TilesParams& p, int grid, int cluster, cudaStream_t st) {
+    const void* fn = reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T>);
+    const int rc = opt_in<kOp, T>();
+    if (rc != A2A_OK) return rc;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t launch{};
+    launch.gridDim = dim3(grid);
+    launch.blockDim = dim3(kTilesThreads);
+    launch.dynamicSmemBytes = kTilesSharedBytes;
+    launch.stream = st;
+    launch.attrs = attr;
+    launch.numAttrs = cluster > 1 ? 2 : 1;
+    void* args[] = {const_cast<TilesParams*>(&p)};
+    const cudaError_t e = cudaLaunchKernelExC(&launch, fn, args);
+    return e == cudaSuccess ? A2A_OK : -(int)e;
+}
+
+// Features of a tile and blocks that share its inner length, for a dense product: what the fullest SM needs least time for. The columns are
+// as many as there are, up to 256.
+struct DensePlan {
+    int height, columns, split;
+};
+template <typename T>
+int most_clusters(int size) {
+    static std::atomic<int> known[kMaxSplit + 1];  // one more than the number; of the first device that asked, as all are alike
+    int n = known[size].load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = size;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t launch{};
+        launch.gridDim = dim3(size);
+        launch.blockDim = dim3(kTilesThreads);
+        launch.dynamicSmemBytes = kTilesSharedBytes;
+        launch.attrs = &attr;
+        launch.numAttrs = 1;
+        if (opt_in<kDense, T>() != A2A_OK || cudaOccupancyMaxActiveClusters(&n, (const void*)&product_tiles_kernel<kDense, T>, &launch) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        known[size].store(++n, std::memory_order_relaxed);
+    }
+    return n - 1;
+}
+
+template <typename T>
+DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
+    const int most = std::min(paired ? kTileRows / 2 : kTileRows, a.outputs), across = parts_of(a.tokens, kMaxColumns);
+    const int columns = std::min(kMaxColumns, round16(parts_of(a.tokens, across))), blocks = parts_of(a.inputs, kTileInner);
+    DensePlan best{most, columns, 1};
+    float least = 1e30f;
+    for (int split = 1; split <= std::min(kMaxSplit, blocks); ++split)
+        for (int height = most; height >= std::min(most, 8); --height) {
+            const int tiles = parts_of(a.outputs, height) * across;
+            // all clusters run at once (they do not come to lie on every SM), or there is nothing to gain
+            if (split > 1 && tiles > most_clusters<T>(split)) break;
+            const int busy = std::min(tiles * split, sms), rounds = split > 1 ? 1 : parts_of(tiles, sms);
+            const float memory = busy / (6500.0f * across), t = rounds * parts_of(blocks, split) * (block_ns(paired ? 2 * height : height, columns, memory) + 15.0f) + (split > 1 ? 1500.0f : 0.0f);
+            if (t < least * 0.999f) least = t, best = DensePlan{height, columns, split};
+        }
+    return best;
 }
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -114,45 +162,31 @@ bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 template <typename T>
 int linear_of(const a2a_linear_args& a, int sms, cudaStream_t st) {
     const bool paired = a.activation == A2A_ACT_SWIGLU;
-    if (a.tokens <= 2 * kRowsTokens) {
-        RowsParams p{};
-        p.weights = a.weight, p.weights_stride = a.weight_stride;
-        p.x = a.x, p.x_stride = a.x_stride;
-        p.inner = a.inputs, p.features = a.outputs, p.tokens = a.tokens;
-        p.activation = a.activation, p.paired = paired, p.out_fp32 = a.out_dtype == A2A_DTYPE_FP32, p.bias_fp32 = a.bias_dtype == A2A_DTYPE_FP32;
-        p.bias = a.bias, p.residual = a.residual, p.residual_stride = a.residual_stride, p.y = a.y, p.y_stride = a.y_stride;
-        const int grid = a.outputs < sms ? a.outputs : sms;
-        return a.tokens <= kRowsTokens ? launch_rows<kRowsDense, T, 1>(p, grid, st) : launch_rows<kRowsDense, T, 2>(p, grid, st);
-    }
     TilesParams p{};
     p.inner = a.inputs, p.features = a.outputs, p.paired = paired, p.groups = 1, p.tokens = a.tokens;
     p.activation = a.activation, p.out_fp32 = a.out_dtype == A2A_DTYPE_FP32, p.bias_fp32 = a.bias_dtype == A2A_DTYPE_FP32;
     p.bias = a.bias, p.residual = a.residual, p.residual_stride = a.residual_stride, p.y = a.y, p.y_stride = a.y_stride;
-    p.columns = a.tokens < kMaxColumns ? (a.tokens + 15) / 16 * 16 : kMaxColumns;
-    int rc = weights_map(&p.weights, a.dtype, a.weight, 1, a.outputs, paired, a.inputs, a.weight_stride);
+    const DensePlan plan = dense_plan<T>(a, paired, sms);
+    p.columns = plan.columns, p.full = plan.height, p.split = plan.split;
+    int rc = weights_map(&p.weights, a.dtype, a.weight, 1, a.outputs, paired, a.inputs, a.weight_stride, plan.height);
     if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.inputs, a.x_stride, p.columns);
     if (rc != A2A_OK) return rc;
-    const int height = paired ? kTileRows / 2 : kTileRows;
-    const long long tiles = (long long)((a.outputs + height - 1) / height) * ((a.tokens + p.columns - 1) / p.columns);
-    return launch_tiles<kDense, T>(p, (int)(tiles < sms ? tiles : sms), st);
+    const int tiles = parts_of(a.outputs, plan.height) * parts_of(a.tokens, plan.columns);
+    return launch_tiles<kDense, T>(p, plan.split > 1 ? tiles * plan.split : std::min(tiles, sms), plan.split, st);
 }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// The workspace of a layer: the experts' inner values, and for more than a few tokens the rows of every pair and the tickets.
+// The workspace of a layer: the experts' inner values, the rows of every pair and the tickets.
 struct LayerSpace {
-    size_t hidden, parts, tickets, end;
+    size_t parts, tickets, end;
 };
 LayerSpace layer_space(int tokens, int topk, int hidden_dim, int inner) {
     LayerSpace s{};
     const size_t pairs = (size_t)tokens * topk;
     s.parts = round256(pairs * inner * 2);
-    if (tokens <= kRowsTokens) {
-        s.tickets = s.end = s.parts;
-    } else {
-        s.tickets = s.parts + round256(pairs * hidden_dim * 4);
-        s.end = s.tickets + round256((size_t)tokens * ((hidden_dim + kTileRows - 1) / kTileRows) * 4);
-    }
+    s.tickets = s.parts + round256(pairs * hidden_dim * 4);
+    s.end = s.tickets + round256((size_t)tokens * parts_of(hidden_dim, kLeastHeight) * 4);
     return s;
 }
 
@@ -161,41 +195,37 @@ bool sizes_fit(int experts, int hidden_dim, int inner) {
            inner % 8 == 0 && inner <= A2A_MAX_PRODUCT;
 }
 
+// Sizes and weights of a launch over experts, in boxes of a whole tile and in pieces.
+int expert_maps(TilesParams& p, int dtype, const void* weights, int experts, int features, bool paired, int inner) {
+    p.inner = inner, p.features = features, p.paired = paired;
+    p.full = std::min(paired ? kTileRows / 2 : kTileRows, features);
+    const int rc = weights_map(&p.weights, dtype, weights, experts, features, paired, inner, inner, p.full);
+    return rc == A2A_OK ? weights_map(&p.weights_piece, dtype, weights, experts, features, paired, inner, inner, kPieceRows / (paired ? 2 : 1)) : rc;
+}
+// Rows that lie in runs.
+int run_maps(TilesParams& p, int dtype, const void* rows, long long count) {
+    const int rc = rows_map(&p.rows, dtype, rows, count, p.inner, p.inner, 64);
+    return rc == A2A_OK ? rows_map(&p.rows_few, dtype, rows, count, p.inner, p.inner, 8) : rc;
+}
+
 template <typename T>
 int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
     uint8_t* const space = static_cast<uint8_t*>(a.workspace);
     const LayerSpace at = layer_space(a.tokens, a.topk, a.hidden_dim, a.inner);
-    if (a.tokens <= kRowsTokens) {
-        RowsParams p{};
-        p.weights = a.gate_up, p.weights_stride = a.hidden_dim;
-        p.x = a.x, p.x_stride = a.hidden_dim;
-        p.inner = a.hidden_dim, p.features = a.inner, p.tokens = a.tokens;
-        p.y = space, p.y_stride = a.inner;
-        p.indices = a.topk_idx, p.weights_of = a.topk_weights, p.topk = a.topk, p.experts = a.experts;
-        const int rc = launch_rows<kRowsUp, T, 1>(p, sms, st);
-        if (rc != A2A_OK) return rc;
-        p.weights = a.down, p.weights_stride = a.inner;
-        p.x = space, p.x_stride = a.inner;
-        p.inner = a.inner, p.features = a.hidden_dim;
-        p.residual = a.residual, p.residual_stride = a.hidden_dim;
-        p.y = a.y, p.y_stride = a.hidden_dim;
-        return launch_rows<kRowsDown, T, 1>(p, a.hidden_dim < sms ? a.hidden_dim : sms, st);
-    }
     TilesParams p{};
     p.groups = a.experts, p.tokens = a.tokens, p.topk = a.topk, p.indices = a.topk_idx, p.weights_of = a.topk_weights;
     p.hidden = space, p.parts = reinterpret_cast<float*>(space + at.parts), p.tickets = reinterpret_cast<int*>(space + at.tickets);
-    p.ticket_count = a.tokens * ((a.hidden_dim + kTileRows - 1) / kTileRows);
+    p.ticket_count = a.tokens * parts_of(a.hidden_dim, kLeastHeight);
     p.columns = kMaxColumns;
-    p.inner = a.hidden_dim, p.features = a.inner, p.paired = 1;
-    int rc = weights_map(&p.weights, a.dtype, a.gate_up, a.experts, a.inner, true, a.hidden_dim, a.hidden_dim);
-    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.hidden_dim, a.hidden_dim, 1);
-    if (rc == A2A_OK) rc = launch_tiles<kLayerUp, T>(p, sms, st);
+    int rc = expert_maps(p, a.dtype, a.gate_up, a.experts, a.inner, true, a.hidden_dim);
+    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.hidden_dim, a.hidden_dim, round16(a.tokens));
+    if (rc == A2A_OK) rc = rows_map(&p.rows_few, a.dtype, a.x, a.tokens, a.hidden_dim, a.hidden_dim, 1);
+    if (rc == A2A_OK) rc = launch_tiles<kLayerUp, T>(p, sms, 1, st);
     if (rc != A2A_OK) return rc;
-    p.inner = a.inner, p.features = a.hidden_dim, p.paired = 0;
     p.residual = a.residual, p.y = a.y;
-    rc = weights_map(&p.weights, a.dtype, a.down, a.experts, a.hidden_dim, false, a.inner, a.inner);
-    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, p.hidden, (long long)a.tokens * a.topk, a.inner, a.inner, 1);
-    return rc == A2A_OK ? launch_tiles<kLayerDown, T>(p, sms, st) : rc;
+    rc = expert_maps(p, a.dtype, a.down, a.experts, a.hidden_dim, false, a.inner);
+    if (rc == A2A_OK) rc = run_maps(p, a.dtype, p.hidden, (long long)a.tokens * a.topk);
+    return rc == A2A_OK ? launch_tiles<kLayerDown, T>(p, sms, 1, st) : rc;
 }
 
 template <typename T>
@@ -204,15 +234,14 @@ int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {
     TilesParams p{};
     p.groups = a.local_experts, p.counts = a.counts, p.world = a.world, p.capacity = a.capacity, p.hidden = a.workspace;
     p.columns = kMaxColumns;
-    p.inner = a.hidden_dim, p.features = a.inner, p.paired = 1;
-    int rc = weights_map(&p.weights, a.dtype, a.gate_up, a.local_experts, a.inner, true, a.hidden_dim, a.hidden_dim);
-    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.rows, rows, a.hidden_dim, a.hidden_dim, 1);
-    if (rc == A2A_OK) rc = launch_tiles<kSlabUp, T>(p, sms, st);
+    int rc = expert_maps(p, a.dtype, a.gate_up, a.local_experts, a.inner, true, a.hidden_dim);
+    if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.rows, rows);
+    if (rc == A2A_OK) rc = launch_tiles<kSlabUp, T>(p, sms, 1, st);
     if (rc != A2A_OK) return rc;
-    p.inner = a.inner, p.features = a.hidden_dim, p.paired = 0, p.y = a.out;
-    rc = weights_map(&p.weights, a.dtype, a.down, a.local_experts, a.hidden_dim, false, a.inner, a.inner);
-    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.workspace, rows, a.inner, a.inner, 1);
-    return rc == A2A_OK ? launch_tiles<kSlabDown, T>(p, sms, st) : rc;
+    p.y = a.out;
+    rc = expert_maps(p, a.dtype, a.down, a.local_experts, a.hidden_dim, false, a.inner);
+    if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.workspace, rows);
+    return rc == A2A_OK ? launch_tiles<kSlabDown, T>(p, sms, 1, st) : rc;
 }
 
 bool dtype16(int dtype) { return dtype == A2A_DTYPE_BF16 || dtype == A2A_DTYPE_FP16; }

@@ -14,17 +14,13 @@
 namespace {
 
 // A wait inside a kernel ends after this long whatever happens: every barrier here is completed by the same block (or its
-// cluster), so one that is not is a fault of this code, and it is to end in an error instead of a GPU that does not answer.
-constexpr long long kWaitNs = 2000000000ll;
+// cluster), so one that is not is a fault of this code, and it is to end in an error instead of a GPU that does not answer. Cycles: two
+// seconds at 2 GHz. (Not the global timer: reading it takes so long that a ring whose every wait did took 0.4 us a step, ten times
+// what the step moved.)
+constexpr long long kWaitCycles = 4000000000ll;
 
 // Set by a kernel whose wait ran out; read and cleared by a2a_product_status.
 __device__ int g_product_error;
-
-__device__ __forceinline__ long long now_ns() {
-    long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
 
 // ---- element types -----------------------------------------------------------------------------
 template <typename T>
@@ -56,7 +52,8 @@ __device__ __forceinline__ void store_any(void* p, size_t i, float v, bool fp32)
 }
 
 // ---- the epilogue's arithmetic: fp32, on the fp32 sums of a product -------------------------------
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
+// (The quick division gives 0 where the divisor is above 2^126: below -87, where silu is less than 1e-35.)
+__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + expf(-v)); }
 
 __device__ __forceinline__ float activate(float v, int activation) {
     switch (activation) {
@@ -68,66 +65,80 @@ __device__ __forceinline__ float activate(float v, int activation) {
     }
 }
 
-// ---- barriers in shared memory -------------------------------------------------------------------
+// ---- barriers in shared memory, by their 32-bit addresses ----------------------------------------------
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void barrier_init(uint64_t* bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_addr(bar)), "r"(count) : "memory");
 }
 __device__ __forceinline__ void barrier_init_done() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
-__device__ __forceinline__ void barrier_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_addr(bar)) : "memory");
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void barrier_expect(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_addr(bar)), "r"(bytes) : "memory");
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(shared_addr(bar)), "r"(parity)
+        : "r"(bar), "r"(parity)
         : "memory");
     return ok != 0;
 }
 
 // Waits for the phase of `parity`; false where the block has given up, or does now because the time has run out.
-__device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
-    if (barrier_try(bar, parity)) return true;
-    const long long begin = now_ns();
+__device__ __noinline__ bool barrier_wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    const long long begin = clock64();
     for (;;) {
-        for (int i = 0; i < 64; ++i)
+        for (int i = 0; i < 16; ++i)
             if (barrier_try(bar, parity)) return true;
         if (*gave_up) return false;
-        if (now_ns() - begin > kWaitNs) {
+        if (clock64() - begin > kWaitCycles) {
             *gave_up = 1;
             return false;
         }
     }
+}
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    return barrier_try(bar, parity) || barrier_wait_long(bar, parity, gave_up);
+}
+
+// True in one lane of the warp, the same one each time. Tensor copies and products are issued under this and not under a test of the lane's
+// number: it tells the compiler that a single thread runs, and their operands go to uniform registers without a loop over lanes.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
 }
 
 // ---- tensor copies, global -> this block's shared memory -------------------------------------------
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-__device__ __forceinline__ void copy_tile_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+__device__ __forceinline__ void copy_tile_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(shared_addr(dst)), "l"(map), "r"(shared_addr(bar)), "r"(x), "r"(y)
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
                  : "memory");
 }
-__device__ __forceinline__ void copy_tile_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+__device__ __forceinline__ void copy_tile_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-        ::"r"(shared_addr(dst)), "l"(map), "r"(shared_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
 // Four rows anywhere in the matrix, one under the other.
-__device__ __forceinline__ void copy_rows_4(void* dst, const CUtensorMap* map, int x, int r0, int r1, int r2, int r3, uint64_t* bar) {
+__device__ __forceinline__ void copy_rows_4(uint32_t dst, const CUtensorMap* map, int x, int r0, int r1, int r2, int r3, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(shared_addr(dst)), "l"(map), "r"(shared_addr(bar)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
         : "memory");
 }
 
@@ -141,8 +152,8 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
 }
 __device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tcgen05_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_addr(bar)) : "memory");
+__device__ __forceinline__ void tcgen05_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tcgen05_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t descriptor, bool add) {
     asm volatile(
@@ -159,19 +170,50 @@ __device__ __forceinline__ void tmem_load_16(uint32_t tmem, float (&v)[16]) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(tmem));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    // the values go through the wait, so that nothing reads them ahead of it
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 16 columns that need not be neighbours: of() gives each one's, the same in all lanes.
+template <typename Of>
+__device__ __forceinline__ void tmem_load_spread(uint32_t tmem, Of of, float (&v)[16]) {
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r[i]) : "r"(tmem + (uint32_t)of(i)));
+    // the values go through the wait, so that nothing reads them ahead of it
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // A K-major operand in shared memory, rows of 128 bytes in the 128-byte swizzle: groups of eight rows are 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand_descriptor(const void* p) {
-    return (uint64_t)((shared_addr(p) & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+__device__ __forceinline__ uint64_t operand_descriptor(uint32_t at) {
+    return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
            (uint64_t)2 << 61;
 }
 // fp32 sums of products of `format` (Element::kFormat), 128 rows by `columns`, both operands K-major.
 __device__ __forceinline__ uint32_t instruction_descriptor(unsigned format, int columns) {
     return 1u << 4 | format << 7 | format << 10 | (uint32_t)(columns >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+}
+
+// All threads of the cluster's blocks meet; what one wrote to its shared memory before, the others see after.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// Where block `rank` of the cluster has what `p` is here.
+template <typename V>
+__device__ __forceinline__ V* cluster_address(V* p, int rank) {
+    V* there;
+    asm volatile("mapa.u64 %0, %1, %2;" : "=l"(there) : "l"(p), "r"(rank));
+    return there;
 }
 
 // Whether all of `threads` threads, which meet here, say yes.

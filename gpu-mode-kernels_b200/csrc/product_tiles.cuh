@@ -1,15 +1,25 @@
 // Products of weights with rows on the tensor cores (tcgen05): y[row] = W x[row], for one matrix and all rows (a dense product) or
 // for a matrix per expert and the rows that chose it.
 //
-// The weights are the operand with 128 rows of a tile, the rows of x its columns: 16 to 256 of them, as many as there are. A decode
-// batch leaves an expert a few rows; a tile of 128 rows of x would be filled to a few per cent, this one moves nothing but weights.
-// Weights come through a ring of tiles in shared memory (tensor copies, 128-byte swizzle), 64 of the inner length at a time; the
-// rows of an expert, which lie anywhere, four at a time by gathering copies into the same stage. Sums are fp32 in tensor memory,
-// two buffers of 256 columns, so that one tile's epilogue runs beside the next one's products.
+// The weights are the operand with 128 rows, the rows of x its columns: 16 to 256 of them, as many as there are. A decode batch leaves
+// an expert a few rows; a tile of 128 rows of x would be filled to a few per cent, this one moves nothing but weights.
+// Weights come through a ring in shared memory (tensor copies, 128-byte swizzle), 64 of the inner length at a time, the rows of x with them.
+// Sums are fp32 in tensor memory, two buffers of 256 columns, so that one tile's epilogue runs beside the next one's products.
 //
-// Roles of the eight warps: 0 weights, 1 products, 2 rows, 3 the lists of rows, 4 to 7 the epilogue.
+// Few rows leave the weights' bytes as the only cost, and then the SMs should have the same number of them: a tile has as many
+// features as makes the number of tiles fill the SMs (`height`), up to what 128 rows hold. Operand rows behind them are whatever lies
+// there; their sums are not read. A dense product with too few features for all SMs is cut along the inner length too, over the blocks
+// of a cluster, which add up their sums in the order of their ranks through distributed shared memory.
 //
-// SwiGLU: a tile is 64 features, their gate and up rows in turn (the tensor map's second dimension steps from gate to up), so that
+// Where rows of x come from: dense, a box of all columns. The first product of a layer: four at a time by gathering copies where an
+// expert has up to 12 rows, else all tokens of the call (at most 256) as columns, of which the expert's are read: a gathering copy of four rows
+// costs 60 to 110 cycles, 43 rows of 173 made a step of 64 take 1230 cycles where the weights' bytes take 700. Everything else
+// lies in runs: boxes of 64 rows, and of 8 at a run's end.
+//
+// Roles of the twelve warps: 0 weights, 1 products, 2 rows, 3 the lists of rows, 4 to 11 the epilogue, two for each 32 lanes of the tensor
+// memory: every other 16 columns each.
+//
+// SwiGLU: a tile's operand rows are gate and up of its features in turn (the tensor map's second dimension steps from gate to up), so that
 // neighbouring lanes of the epilogue hold the two and exchange by shuffles.
 #pragma once
 
@@ -20,21 +30,32 @@ namespace {
 enum TilesOp { kDense, kLayerUp, kLayerDown, kSlabUp, kSlabDown };
 
 constexpr int kTileRows = 128, kTileInner = 64, kMaxColumns = 256;
-constexpr int kTilesThreads = 256;
+constexpr int kRowBytes = kTileInner * 2;
+constexpr int kTilesThreads = 384, kFinishers = 256;  // of which the epilogue's
 constexpr int kRingBytes = 192 * 1024, kMaxStages = 12;
+constexpr int kStageBytes = 32 * 1024;  // a stage has as many blocks of 64 as reach this, so that small tiles do not pay a barrier for each
 constexpr int kMaxGroups = A2A_MAX_EXPERTS;
 constexpr int kTmemColumns = 512;
+constexpr int kGathered = 12;     // most rows of an expert that are gathered
+constexpr int kPieceRows = 32;    // operand rows of a box of a tile that is less than full
+constexpr int kLeastHeight = kPieceRows;  // features of a tile of kLayerDown at least: there is a ticket for each token and tile
+constexpr int kMaxSplit = 8;
 
 struct TilesParams {
-    CUtensorMap weights;  // [groups][rows or features][1 or gate, up][inner], boxes of 128 rows by 64
-    CUtensorMap rows;     // kDense: boxes of `columns` rows by 64; else of one row, for gathering
-    int inner;            // length of a sum
-    int features;         // of the output, per group
-    int paired;           // SwiGLU
-    int groups;           // matrices
-    int columns;          // most columns a tile may have
-    // kDense: rows of x, and the epilogue
-    int tokens, activation, out_fp32, bias_fp32;
+    CUtensorMap weights;        // [groups][features][1 or gate, up][inner], boxes of `full` features by 64
+    CUtensorMap weights_piece;  // the same in boxes of kPieceRows operand rows; not kDense
+    CUtensorMap rows;           // boxes of 64 of the inner length by: kDense `columns` rows, kLayerUp all tokens, else 64 rows
+    CUtensorMap rows_few;       // kLayerUp: a row, for gathering; else 8 rows; not kDense
+    int inner;                  // length of a sum
+    int features;               // of the output, per group
+    int paired;                 // SwiGLU
+    int groups;                 // matrices
+    int full;                   // most features a tile may have; kDense: what it has
+    int columns;                // most columns a tile may have
+    int split;                  // kDense: blocks of a cluster, which share a tile's inner length
+    int tokens;
+    // kDense: the epilogue
+    int activation, out_fp32, bias_fp32;
     const void* bias;
     const void* residual;  // also kLayerDown
     long long residual_stride;
@@ -44,9 +65,9 @@ struct TilesParams {
     const int* indices;
     const float* weights_of;
     int topk;
-    void* hidden;   // [row][features] of *Up
-    float* parts;   // [pair][features] of kLayerDown
-    int* tickets;   // [token][tile of features] of kLayerDown, zeroed by kLayerUp
+    void* hidden;  // kLayerUp: [pair, by expert][features]; kSlabUp: [row of the slabs][features]
+    float* parts;  // [pair][features] of kLayerDown
+    int* tickets;  // [token][tile of features] of kLayerDown, zeroed by kLayerUp
     int ticket_count;
     // kSlab*
     const int* counts;
@@ -59,32 +80,49 @@ struct TilesShared {
     uint64_t list_full[2], list_empty[2];
     uint32_t tmem;
     int gave_up;
-    int largest;    // rows of the largest group
+    int largest;  // columns of the largest group
     int last_count;
-    int begin[kMaxGroups + 1];  // first tile of a group
-    int count[kMaxGroups];      // its rows
-    int list[2][kMaxColumns];
+    int height;
+    int begin[kMaxGroups + 1];  // tiles of one feature tile before a group's
+    int count[kMaxGroups];      // columns of a group
+    int row[kMaxGroups];        // rows before a group's (kLayer*)
+    int list[2][kMaxColumns];   // columns of a tile: pair (kLayer*) or row of the slabs, -1 for none
     float scale[2][kMaxColumns];
     int last[kMaxColumns];
+    alignas(16) int2 box[2][kMaxColumns / 8];  // kSlab*: first row and twice the first column, plus one if it is of 64 rows
+    int boxes[2];
+    // What an operand of less than 128 rows at the end of the ring is read beyond it.
+    uint8_t behind[2048];
 };
+static_assert(sizeof(TilesShared) >= kTileRows * kRowBytes, "operands of 128 rows end within the shared memory");
 
 constexpr size_t kTilesSharedBytes = 1024 + kRingBytes + sizeof(TilesShared);
 static_assert(kTilesSharedBytes <= 227 * 1024, "a block's shared memory");
 
 struct Tile {
-    int group, m, first, columns;  // matrix, tile of its features, first row, rows
+    int group, m, first, columns;  // matrix, tile of its features, first column, columns
 };
 
-__device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
+__host__ __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
+__host__ __device__ __forceinline__ int parts_of(int n, int size) { return (n + size - 1) / size; }
+
+// What a block of 64 of a tile takes, in ns: the SM's share of the memory's rate for the weights (6.5 TB/s over 148), what the L2 gives an SM
+// (90 bytes a ns), or the products (256 columns by 64 in 512 cycles).
+__host__ __device__ __forceinline__ float block_ns(int rows, int columns, float memory_share) {
+    const float memory = rows * kRowBytes * memory_share, cache = (rows + columns) * kRowBytes * (1.0f / 90), products = columns * 1.05f;
+    return fmaxf(fmaxf(memory, cache), products);
+}
 
 template <TilesOp kOp, typename T>
 __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const __grid_constant__ TilesParams p) {
-    constexpr bool kGrouped = kOp != kDense, kLayer = kOp == kLayerUp || kOp == kLayerDown;
+    constexpr bool kGrouped = kOp != kDense, kLayer = kOp == kLayerUp || kOp == kLayerDown, kSlab = kOp == kSlabUp || kOp == kSlabDown;
     constexpr bool kFirst = kOp == kDense || kOp == kLayerUp || kOp == kSlabUp;  // nothing of the same call runs before it
+    constexpr bool kUp = kOp == kLayerUp || kOp == kSlabUp;
     extern __shared__ uint8_t shared_raw[];
     uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(shared_raw) + 1023) & ~(uintptr_t)1023);
     TilesShared& s = *reinterpret_cast<TilesShared*>(ring + kRingBytes);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool paired = kUp || (kOp == kDense && p.paired);
 
     if (tid == 0) {
         for (int i = 0; i < kMaxStages; ++i) {
@@ -93,33 +131,32 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         }
         for (int i = 0; i < 2; ++i) {
             barrier_init(&s.sums_full[i], 1);
-            barrier_init(&s.sums_empty[i], 4);
+            barrier_init(&s.sums_empty[i], kFinishers / 32);
             barrier_init(&s.list_full[i], 1);
-            barrier_init(&s.list_empty[i], 2);
+            barrier_init(&s.list_empty[i], kOp == kLayerDown ? 1 : 2);  // the roles that read it
         }
         s.gave_up = s.largest = s.last_count = 0;
         barrier_init_done();
-        prefetch_map(&p.weights);
-        prefetch_map(&p.rows);
     }
     if (warp == 1) tmem_alloc(&s.tmem, kTmemColumns);
+    if (warp == 2 && lane < (kGrouped ? 4 : 2))
+        prefetch_map(lane == 0 ? &p.weights : lane == 1 ? &p.rows : lane == 2 ? &p.weights_piece : &p.rows_few);
     // The second product of a call reads weights, indices and counts ahead of this: what wrote those was through before the
     // first product let this launch begin.
     if (kFirst) {
         cudaGridDependencySynchronize();
         cudaTriggerProgrammaticLaunchCompletion();
     }
-    const int feature_tiles = (p.features + (p.paired ? kTileRows / 2 : kTileRows) - 1) / (p.paired ? kTileRows / 2 : kTileRows);
     if (kOp == kLayerUp)
         for (int i = blockIdx.x * kTilesThreads + tid; i < p.ticket_count; i += gridDim.x * kTilesThreads) p.tickets[i] = 0;
 
-    // ---- how many rows every group has, and so the tiles ----
-    int columns = p.columns;
+    // ---- how many columns every group has, and so the tiles ----
+    int columns = p.columns, height = p.full;
     if (kGrouped) {
         for (int g = tid; g < p.groups; g += kTilesThreads) {
             int n = 0;
-            if (!kLayer)
-                for (int src = 0; src < p.world; ++src) n += min(max(p.counts[(size_t)src * 4 * p.groups + g], 0), p.capacity);
+            if (kSlab)  // a rank's rows in whole boxes of eight
+                for (int src = 0; src < p.world; ++src) n += (min(max(p.counts[(size_t)src * 4 * p.groups + g], 0), p.capacity) + 7) & ~7;
             s.count[g] = n;
         }
         __syncthreads();
@@ -134,153 +171,213 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0) atomicMax(&s.largest, most);
         __syncthreads();
-        columns = min(columns, max(16, round16(s.largest)));
+        columns = min(p.columns, max(16, round16(s.largest)));
         if (warp == 0) {
-            int run = 0;
+            int run = 0, rows = 0;
             for (int g0 = 0; g0 < p.groups; g0 += 32) {
-                const int g = g0 + lane;
-                const int own = g < p.groups ? (s.count[g] + columns - 1) / columns * feature_tiles : 0;
-                int sum = own;
+                const int g = g0 + lane, n = g < p.groups ? s.count[g] : 0;
+                const int own = parts_of(n, columns);
+                int sum = own, sum_rows = n;
                 for (int d = 1; d < 32; d <<= 1) {
-                    const int left = __shfl_up_sync(0xffffffffu, sum, d);
-                    if (lane >= d) sum += left;
+                    const int left = __shfl_up_sync(0xffffffffu, sum, d), left_rows = __shfl_up_sync(0xffffffffu, sum_rows, d);
+                    if (lane >= d) sum += left, sum_rows += left_rows;
                 }
-                if (g < p.groups) s.begin[g] = run + sum - own;
+                if (g < p.groups) s.begin[g] = run + sum - own, s.row[g] = rows + sum_rows - n;
                 run += __shfl_sync(0xffffffffu, sum, 31);
+                rows += __shfl_sync(0xffffffffu, sum_rows, 31);
             }
-            if (lane == 0) s.begin[p.groups] = run;
+            // the height whose tiles take the fullest SM least: whole boxes, or a lane a number of pieces
+            const int piece = kPieceRows / (kUp ? 2 : 1), h = lane == 31 ? p.full : piece * (lane + 1);
+            unsigned cost = 0xffffffffu;
+            if (h < p.full || lane == 31) {
+                const int wide = kOp == kLayerUp && s.largest > kGathered ? round16(p.tokens) : columns;
+                const int rounds = parts_of(run * parts_of(p.features, h), gridDim.x);
+                cost = (unsigned)fminf(rounds * (block_ns(h * (kUp ? 2 : 1), wide, 1.0f / 44) + 10.0f) * 8.0f, 1e9f);
+            }
+            const unsigned least = __reduce_min_sync(0xffffffffu, cost);
+            const int best = 31 - __clz(__ballot_sync(0xffffffffu, cost == least));  // the highest of the best
+            if (lane == 0) s.begin[p.groups] = run, s.height = best == 31 ? p.full : piece * (best + 1);
         }
     }
     tcgen05_before_sync();
     __syncthreads();
     tcgen05_after_sync();
+    if (kGrouped) height = s.height;
     const uint32_t tmem = s.tmem;
-    const int tiles = kGrouped ? s.begin[p.groups] : (p.tokens + columns - 1) / columns * feature_tiles;
-    const int stage_bytes = kTileRows * 128 + columns * 128;
-    const int stages = min(kMaxStages, kRingBytes / stage_bytes);
-    const int steps = (p.inner + kTileInner - 1) / kTileInner;
+    const uint32_t full0 = shared_addr(s.full), empty0 = shared_addr(s.empty), sums_full0 = shared_addr(s.sums_full), sums_empty0 = shared_addr(s.sums_empty),
+                   list_full0 = shared_addr(s.list_full), list_empty0 = shared_addr(s.list_empty), ring0 = shared_addr(ring);
+    const int feature_tiles = parts_of(p.features, height);
+    const int across_all = kGrouped ? s.begin[p.groups] : parts_of(p.tokens, columns);
+    const int tiles = across_all * feature_tiles;
+    // the operand's columns in a stage
+    const int wide = kOp == kLayerUp ? (s.largest > kGathered ? round16(p.tokens) : 16) : columns;
+    const int operand_rows = paired ? 2 * height : height;
+    const int weight_bytes = (operand_rows * kRowBytes + 1023) & ~1023, block_bytes = weight_bytes + wide * kRowBytes;
+    const int blocks_all = parts_of(p.inner, kTileInner);
+    const int per_stage = min(blocks_all, max(1, (kStageBytes + block_bytes / 2) / block_bytes));
+    const int stages = min(kMaxStages, kRingBytes / (block_bytes * per_stage));
+    // this block's part of the inner length, and its tiles
+    const int split = kOp == kDense ? p.split : 1, part = kOp == kDense ? (int)blockIdx.x % split : 0;
+    const int block0 = blocks_all * part / split, blocks = blocks_all * (part + 1) / split - block0;
+    const int steps = parts_of(blocks, per_stage);
+    const int tile0 = (int)blockIdx.x / split, tile_step = (int)gridDim.x / split;
 
     // Tiles that share weights come one after the other, so that blocks read them together.
     auto tile_of = [&](int t) {
         Tile x;
-        int rows;
+        int count;
         if (kGrouped) {
-            int lo = 0, hi = p.groups - 1;  // the last group that begins at or before t; groups without rows begin with the next
+            const int q = t / feature_tiles;
+            int lo = 0, hi = p.groups - 1;  // the last group that begins at or before q; groups without rows begin with the next
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
-                if (s.begin[mid] <= t) lo = mid;
+                if (s.begin[mid] <= q) lo = mid;
                 else hi = mid - 1;
             }
             x.group = lo;
-            rows = s.count[lo];
-            t -= s.begin[lo];
+            count = s.count[lo];
+            t -= s.begin[lo] * feature_tiles;
         } else {
             x.group = 0;
-            rows = p.tokens;
+            count = p.tokens;
         }
-        const int across = (rows + columns - 1) / columns;
+        const int across = parts_of(count, columns);
         x.m = t / across;
         x.first = (t - x.m * across) * columns;
-        x.columns = min(columns, rows - x.first);
+        x.columns = min(columns, count - x.first);
         return x;
     };
+    // kLayerUp: whether all tokens are this tile's columns
+    auto all_tokens = [&](const Tile& x) { return kOp == kLayerUp && s.count[x.group] > kGathered; };
 
+    const uint32_t stage_bytes = (uint32_t)per_stage * block_bytes;
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             int stage = 0;
             uint32_t phase = 1;
-            for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+            const bool whole = !kGrouped || height == p.full;  // a box of all features, or pieces
+            const int piece = kPieceRows / (paired ? 2 : 1);
+            for (int t = tile0; t < tiles; t += tile_step) {
                 const Tile x = tile_of(t);
-                const int f = x.m * (p.paired ? kTileRows / 2 : kTileRows);
-                for (int i = 0; i < steps; ++i) {
-                    if (!barrier_wait(&s.empty[stage], phase, &s.gave_up)) goto weights_done;
-                    barrier_expect(&s.full[stage], kTileRows * 128);
-                    copy_tile_4d(ring + stage * stage_bytes, &p.weights, i * kTileInner, 0, f, x.group, &s.full[stage]);
+                const int f = x.m * height;
+                int k = block0 * kTileInner;
+                for (int left = blocks; left > 0; left -= per_stage) {
+                    const uint32_t bar = full0 + 8 * stage;
+                    uint32_t at = ring0 + stage * stage_bytes;
+                    if (!barrier_wait(empty0 + 8 * stage, phase, &s.gave_up)) goto weights_done;
+                    int n = min(per_stage, left);
+                    barrier_expect(bar, n * operand_rows * kRowBytes);
+                    for (; n > 0; --n, k += kTileInner, at += block_bytes) {
+                        if (whole) {
+                            copy_tile_4d(at, &p.weights, k, 0, f, x.group, bar);
+                        } else {
+                            uint32_t to = at;
+                            for (int h = 0; h < height; h += piece, to += kPieceRows * kRowBytes) copy_tile_4d(to, &p.weights_piece, k, 0, f + h, x.group, bar);
+                        }
+                    }
                     if (++stage == stages) stage = 0, phase ^= 1;
                 }
             }
         weights_done:;
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             int stage = 0, n = 0;
             uint32_t phase = 0;
-            for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+            const uint64_t ring_descriptor = operand_descriptor(ring0);
+            for (int t = tile0; t < tiles; t += tile_step, ++n) {
                 const Tile x = tile_of(t);
                 const int buffer = n & 1;
-                const uint32_t descriptor = instruction_descriptor(Element<T>::kFormat, round16(x.columns));
-                if (!barrier_wait(&s.sums_empty[buffer], ((n >> 1) & 1) ^ 1, &s.gave_up)) goto products_done;
+                const uint32_t descriptor = instruction_descriptor(Element<T>::kFormat, round16(all_tokens(x) ? p.tokens : x.columns));
+                const uint32_t sums = tmem + buffer * kMaxColumns;
+                if (!barrier_wait(sums_empty0 + 8 * buffer, ((n >> 1) & 1) ^ 1, &s.gave_up)) goto products_done;
                 tcgen05_after_sync();
-                for (int i = 0; i < steps; ++i) {
-                    if (!barrier_wait(&s.full[stage], phase, &s.gave_up)) goto products_done;
-                    tcgen05_after_sync();
-                    const uint64_t a = operand_descriptor(ring + stage * stage_bytes);
-                    const uint64_t b = operand_descriptor(ring + stage * stage_bytes + kTileRows * 128);
-#pragma unroll
-                    for (int k = 0; k < kTileInner / 16; ++k)  // 16 of the inner length are 32 bytes of a row
-                        tcgen05_mma(tmem + buffer * kMaxColumns, a + 2 * k, b + 2 * k, descriptor, i + k > 0);
-                    tcgen05_commit(&s.empty[stage]);
+                bool add = false;
+                for (int left = blocks; left > 0; left -= per_stage) {
+                    uint64_t w = ring_descriptor + (stage * stage_bytes >> 4);
+                    if (!barrier_wait(full0 + 8 * stage, phase, &s.gave_up)) goto products_done;
+                    for (int b = min(per_stage, left); b > 0; --b, w += block_bytes >> 4) {
+                        const uint64_t r = w + (weight_bytes >> 4);
+                        // 16 of the inner length are 32 bytes of a row
+                        tcgen05_mma(sums, w, r, descriptor, add);
+                        tcgen05_mma(sums, w + 2, r + 2, descriptor, true);
+                        tcgen05_mma(sums, w + 4, r + 4, descriptor, true);
+                        tcgen05_mma(sums, w + 6, r + 6, descriptor, true);
+                        add = true;
+                    }
+                    tcgen05_commit(empty0 + 8 * stage);
                     if (++stage == stages) stage = 0, phase ^= 1;
                 }
-                tcgen05_commit(&s.sums_full[buffer]);
+                tcgen05_commit(sums_full0 + 8 * buffer);
             }
         products_done:;
         }
     } else if (warp == 2) {
         if (!kFirst) cudaGridDependencySynchronize();
-        int stage = 0, n = 0;
-        uint32_t phase = 1;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
-            const Tile x = tile_of(t);
-            if (!kGrouped) {
-                if (lane == 0)
-                    for (int i = 0; i < steps; ++i) {
-                        if (!barrier_wait(&s.empty[stage], phase, &s.gave_up)) break;
-                        barrier_expect(&s.full[stage], columns * 128);
-                        copy_tile_2d(ring + stage * stage_bytes + kTileRows * 128, &p.rows, i * kTileInner, x.first, &s.full[stage]);
-                        if (++stage == stages) stage = 0, phase ^= 1;
+        if (elect_one()) {
+            int stage = 0, n = 0;
+            uint32_t phase = 1;
+            for (int t = tile0; t < tiles; t += tile_step, ++n) {
+                const Tile x = tile_of(t);
+                // the tile's copies of a block of 64: one box, or four rows at a time, or boxes of eight rows and of 64
+                int bytes = wide * kRowBytes, four[kGathered], boxes = 0;
+                bool box = kOp == kDense;
+                if (kOp == kLayerDown) {
+                    bytes = (x.columns + 7 & ~7) * kRowBytes;
+                } else if (kOp != kDense) {
+                    if (!barrier_wait(list_full0 + 8 * (n & 1), (n >> 1) & 1, &s.gave_up)) goto rows_done;
+                    if (kSlab) {
+                        bytes = x.columns * kRowBytes;
+                        boxes = s.boxes[n & 1];
+                    } else if (all_tokens(x)) {
+                        box = true;
+                    } else {
+                        bytes = (x.columns + 3 & ~3) * kRowBytes;
+                        // Behind the last row the first one stands again: its sums are not read.
+#pragma unroll
+                        for (int j = 0; j < kGathered; ++j) four[j] = s.list[n & 1][j < x.columns ? j : 0] / p.topk;
                     }
-                if (s.gave_up) break;
-                continue;
-            }
-            const int buffer = n & 1;
-            if (!__all_sync(0xffffffffu, barrier_wait(&s.list_full[buffer], (n >> 1) & 1, &s.gave_up))) break;
-            // Lane i's rows 4 i to 4 i + 3 and, of more than 128, the same further on. Behind the last row the first one stands
-            // again: its sums are not read.
-            int r[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int c = 128 * h + 4 * lane + j;
-                    const int row = s.list[buffer][c < x.columns ? c : 0];
-                    r[h][j] = kOp == kLayerUp ? row / p.topk : row;
                 }
-            __syncwarp();
-            if (lane == 0) barrier_arrive(&s.list_empty[buffer]);
-            const int fours = (x.columns + 3) >> 2;
-            bool ok = true;
-            for (int i = 0; i < steps; ++i) {
-                ok = __all_sync(0xffffffffu, barrier_wait(&s.empty[stage], phase, &s.gave_up));
-                if (!ok) break;
-                if (lane == 0) barrier_expect(&s.full[stage], fours * 512);
-                __syncwarp();
-                uint8_t* const at = ring + stage * stage_bytes + kTileRows * 128;
+                int k = block0 * kTileInner;
+                for (int left = blocks; left > 0; left -= per_stage) {
+                    const uint32_t bar = full0 + 8 * stage;
+                    uint32_t at = ring0 + stage * stage_bytes + weight_bytes;
+                    if (!barrier_wait(empty0 + 8 * stage, phase, &s.gave_up)) goto rows_done;
+                    int have = min(per_stage, left);
+                    barrier_expect(bar, have * bytes);
+                    for (; have > 0; --have, k += kTileInner, at += block_bytes) {
+                        if (kOp == kDense || (kOp == kLayerUp && box)) {
+                            copy_tile_2d(at, &p.rows, k, kOp == kDense ? x.first : 0, bar);
+                        } else if (kOp == kLayerUp) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (32 * h + lane < fours)
-                        copy_rows_4(at + (32 * h + lane) * 512, &p.rows, i * kTileInner, r[h][0], r[h][1], r[h][2], r[h][3], &s.full[stage]);
-                if (++stage == stages) stage = 0, phase ^= 1;
+                            for (int j = 0; j < kGathered; j += 4)
+                                if (j < x.columns) copy_rows_4(at + j * kRowBytes, &p.rows_few, k, four[j], four[j + 1], four[j + 2], four[j + 3], bar);
+                        } else if (kOp == kLayerDown) {
+                            int c = 0;
+                            const int first = s.row[x.group] + x.first;  // the inner values lie by expert
+                            for (; c + 64 <= x.columns; c += 64) copy_tile_2d(at + c * kRowBytes, &p.rows, k, first + c, bar);
+                            for (; c < x.columns; c += 8) copy_tile_2d(at + c * kRowBytes, &p.rows_few, k, first + c, bar);
+                        } else {
+                            for (int j = 0; j < boxes; j += 2) {
+                                const int4 two = *reinterpret_cast<const int4*>(&s.box[n & 1][j]);
+                                copy_tile_2d(at + (two.y >> 1) * kRowBytes, two.y & 1 ? &p.rows : &p.rows_few, k, two.x, bar);
+                                if (j + 1 < boxes) copy_tile_2d(at + (two.w >> 1) * kRowBytes, two.w & 1 ? &p.rows : &p.rows_few, k, two.z, bar);
+                            }
+                        }
+                    }
+                    if (++stage == stages) stage = 0, phase ^= 1;
+                }
+                if (kOp == kLayerUp || kSlab) barrier_arrive(list_empty0 + 8 * (n & 1));
             }
-            if (!ok) break;
+        rows_done:;
         }
     } else if (warp == 3) {
         if (kGrouped) {
             int n = 0;
-            for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+            for (int t = tile0; t < tiles; t += tile_step, ++n) {
                 const Tile x = tile_of(t);
                 const int buffer = n & 1;
-                if (!__all_sync(0xffffffffu, barrier_wait(&s.list_empty[buffer], ((n >> 1) & 1) ^ 1, &s.gave_up))) break;
+                if (!__all_sync(0xffffffffu, barrier_wait(list_empty0 + 8 * buffer, ((n >> 1) & 1) ^ 1, &s.gave_up))) break;
                 if (kLayer) {
                     // pairs in ascending order: which tile of a group a pair belongs to is the same for every block
                     const int pairs = p.tokens * p.topk;
@@ -306,29 +403,42 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     }
                 } else {
                     for (int c = lane; c < x.columns; c += 32) {
-                        int r = x.first + c, src = 0;
-                        for (;;) {
-                            const int have = min(max(p.counts[(size_t)src * 4 * p.groups + x.group], 0), p.capacity);
-                            if (r < have || src == p.world - 1) break;
-                            r -= have;
-                            ++src;
+                        int r = x.first + c, src = 0, have = 0;
+                        for (; src < p.world; ++src) {
+                            have = min(max(p.counts[(size_t)src * 4 * p.groups + x.group], 0), p.capacity);
+                            const int room = (have + 7) & ~7;
+                            if (r < room) break;
+                            r -= room;
                         }
-                        s.list[buffer][c] = (x.group * p.world + src) * p.capacity + min(r, p.capacity - 1);
+                        s.list[buffer][c] = src < p.world && r < have ? (x.group * p.world + src) * p.capacity + r : -1;
                     }
+                    __syncwarp();
+                    // Boxes of eight rows, a lane each (every eight columns begin with a row); eight of them in one run are one box.
+                    const int eights = x.columns >> 3, row = lane < eights ? s.list[buffer][8 * lane] : -1;
+                    const int before = __shfl_up_sync(0xffffffffu, row, 1);
+                    const unsigned breaks = __ballot_sync(0xffffffffu, lane == 0 || lane >= eights || row != before + 8);
+                    const int run0 = 31 - __clz(breaks & (0xffffffffu >> (31 - lane)));        // where this lane's run begins
+                    const unsigned later = lane == 31 ? 0 : breaks >> (lane + 1);
+                    const int run1 = later ? lane + __ffs(later) : 32;                           // and ends
+                    const int place = (lane - run0) & 7, wide_boxes = (run1 - run0) >> 3;
+                    const bool is_wide = (lane - run0) >> 3 < wide_boxes, issues = lane < eights && (!is_wide || place == 0);
+                    const unsigned issuing = __ballot_sync(0xffffffffu, issues);
+                    if (issues) s.box[buffer][__popc(issuing & ((1u << lane) - 1))] = make_int2(row, 8 * lane << 1 | (is_wide ? 1 : 0));
+                    if (lane == 0) s.boxes[buffer] = __popc(issuing);
                 }
                 __syncwarp();
-                if (lane == 0) barrier_arrive(&s.list_full[buffer]);
+                if (lane == 0) barrier_arrive(list_full0 + 8 * buffer);
             }
         }
     } else {
-        const int quarter = warp - 4, at = tid - 128;
+        const int quarter = warp & 3, half = (warp - 4) >> 2, at = tid - 128;
         if (!kFirst) {
             cudaGridDependencySynchronize();
             cudaTriggerProgrammaticLaunchCompletion();
         }
         if (kOp == kLayerDown) {
             // tokens that no expert of the layer was chosen for: nobody below draws a ticket for them
-            for (int token = blockIdx.x * 4 + quarter; token < p.tokens; token += gridDim.x * 4) {
+            for (int token = blockIdx.x * (kFinishers / 32) + warp - 4; token < p.tokens; token += gridDim.x * (kFinishers / 32)) {
                 const int e = lane < p.topk ? p.indices[token * p.topk + lane] : -1;
                 if (__any_sync(0xffffffffu, e >= 0 && e < p.groups)) continue;
                 for (int f = lane; f < p.features; f += 32)
@@ -337,80 +447,120 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             }
         }
         int n = 0;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+        bool met = kOp != kDense || split == 1;
+        for (int t = tile0; t < tiles; t += tile_step, ++n) {
             const Tile x = tile_of(t);
             const int buffer = n & 1;
-            bool here = !kGrouped || barrier_wait(&s.list_full[buffer], (n >> 1) & 1, &s.gave_up);
-            here = here && barrier_wait(&s.sums_full[buffer], (n >> 1) & 1, &s.gave_up);
-            if (!named_all(1, 128, here)) break;  // all four warps go on, or none
+            bool here = !kGrouped || barrier_wait(list_full0 + 8 * buffer, (n >> 1) & 1, &s.gave_up);
+            here = here && barrier_wait(sums_full0 + 8 * buffer, (n >> 1) & 1, &s.gave_up);
+            if (!named_all(1, kFinishers, here)) break;  // all warps go on, or none
             tcgen05_after_sync();
             const uint32_t sums = tmem + buffer * kMaxColumns + ((uint32_t)(quarter * 32) << 16);
-            // this lane's feature, and its row of the weights
-            const int f = p.paired ? x.m * (kTileRows / 2) + quarter * 16 + (lane >> 1) : x.m * kTileRows + quarter * 32 + lane;
-            const bool inside = f < p.features;
+            // this lane's feature
+            const int own = quarter * 32 + lane, within = paired ? own >> 1 : own, f = x.m * height + within;
+            const bool inside = within < height && f < p.features, up = paired && (lane & 1);
+            const bool needed = (paired ? quarter * 16 : quarter * 32) < height;  // by warp
             float bias = 0.0f;
             if (kOp == kDense && p.bias != nullptr && inside)
-                bias = load_any<T>(p.bias, p.paired ? (size_t)(lane & 1) * p.features + f : f, p.bias_fp32);
-            for (int c0 = 0; c0 < x.columns; c0 += 16) {
-                float v[16];
-                tmem_load_16(sums + c0, v);
-                if (p.paired) {
-                    // lanes 2 i and 2 i + 1 hold gate and up of a feature: the first finishes the even columns, the second the odd ones
-                    const bool up = lane & 1;
+                bias = load_any<T>(p.bias, (size_t)(up ? p.features : 0) + f, p.bias_fp32);
+            // Finishes columns c0 to c0 + kCount - 1 (an even number). With SwiGLU lanes 2 i and 2 i + 1 hold gate and up of a feature: the
+            // first finishes the even columns, the second the odd ones. Values first, then the stores, so that the columns overlap.
+            auto finish = [&](int c0, auto& v) {
+                constexpr int kCount = sizeof(v) / sizeof(float);
+                if (paired) {
+                    float out[kCount / 2], add[kCount / 2];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < kCount / 2; ++j) {
+                        const int c = c0 + 2 * j + up;
+                        add[j] = 0.0f;
+                        if (kOp == kDense && p.residual != nullptr && inside && c < x.columns)
+                            add[j] = load_any<T>(p.residual, (size_t)(x.first + c) * p.residual_stride + f, p.out_fp32);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kCount / 2; ++j) {
                         const float even = v[2 * j] + bias, odd = v[2 * j + 1] + bias;
                         const float other = __shfl_xor_sync(0xffffffffu, up ? even : odd, 1);
-                        const float gate = up ? other : even, lift = up ? odd : other;
-                        v[j] = silu(gate) * lift;
+                        out[j] = silu(up ? other : even) * (up ? odd : other) + add[j];
                     }
+                    if (!inside) return;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int c = c0 + 2 * j + (up ? 1 : 0);
-                        if (!inside || c >= x.columns) continue;
+                    for (int j = 0; j < kCount / 2; ++j) {
+                        const int c = c0 + 2 * j + up;
+                        if (c >= x.columns) continue;
                         if (kOp == kDense) {
-                            const size_t token = x.first + c;
-                            const float r = p.residual != nullptr ? load_any<T>(p.residual, token * p.residual_stride + f, p.out_fp32) : 0.0f;
-                            store_any<T>(p.y, token * p.y_stride + f, v[j] + r, p.out_fp32);
+                            store_any<T>(p.y, (size_t)(x.first + c) * p.y_stride + f, out[j], p.out_fp32);
                         } else {
                             // Rounded to the rows' type, since the next product takes 16-bit operands.
-                            static_cast<T*>(p.hidden)[(size_t)s.list[buffer][c] * p.features + f] = Element<T>::from_float(v[j]);
+                            const int row = kOp == kLayerUp ? s.row[x.group] + x.first + c : s.list[buffer][c];
+                            if (row >= 0) static_cast<T*>(p.hidden)[(size_t)row * p.features + f] = Element<T>::from_float(out[j]);
                         }
                     }
+                    return;
+                }
+                if (!inside) return;
+                if (kOp == kDense) {
+                    float add[kCount];
+#pragma unroll
+                    for (int j = 0; j < kCount; ++j) {
+                        add[j] = 0.0f;
+                        if (p.residual != nullptr && c0 + j < x.columns)
+                            add[j] = load_any<T>(p.residual, (size_t)(x.first + c0 + j) * p.residual_stride + f, p.out_fp32);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kCount; ++j) add[j] += activate(v[j] + bias, p.activation);
+#pragma unroll
+                    for (int j = 0; j < kCount; ++j)
+                        if (c0 + j < x.columns) store_any<T>(p.y, (size_t)(x.first + c0 + j) * p.y_stride + f, add[j], p.out_fp32);
                 } else {
-                    float r[16];
-                    if (kOp == kDense && p.residual != nullptr) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            r[j] = inside && c0 + j < x.columns
-                                       ? load_any<T>(p.residual, (size_t)(x.first + c0 + j) * p.residual_stride + f, p.out_fp32)
-                                       : 0.0f;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
+                    for (int j = 0; j < kCount; ++j) {
                         const int c = c0 + j;
-                        if (!inside || c >= x.columns) continue;
-                        if (kOp == kDense) {
-                            float out = activate(v[j] + bias, p.activation);
-                            if (p.residual != nullptr) out += r[j];
-                            store_any<T>(p.y, (size_t)(x.first + c) * p.y_stride + f, out, p.out_fp32);
-                        } else if (kOp == kLayerDown) {
-                            p.parts[(size_t)s.list[buffer][c] * p.features + f] = s.scale[buffer][c] * v[j];
-                        } else {
-                            static_cast<T*>(p.y)[(size_t)s.list[buffer][c] * p.features + f] = Element<T>::from_float(v[j]);
-                        }
+                        if (c >= x.columns) break;
+                        const int row = s.list[buffer][c];
+                        if (kOp == kLayerDown) p.parts[(size_t)row * p.features + f] = s.scale[buffer][c] * v[j];
+                        else if (row >= 0) static_cast<T*>(p.y)[(size_t)row * p.features + f] = Element<T>::from_float(v[j]);
                     }
+                }
+            };
+            if (kOp == kDense && split > 1) {
+                // The cluster's blocks leave their sums in the ring, which nothing uses any more, and each finishes its share of the
+                // columns, two at a time.
+                float* const left = reinterpret_cast<float*>(ring);
+                for (int c0 = 16 * half; c0 < x.columns && needed; c0 += 32) {
+                    float v[16];
+                    tmem_load_16(sums + c0, v);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) left[(c0 + j) * kTileRows + own] = v[j];
+                }
+                cluster_sync();
+                met = true;
+                for (int c = 2 * (part + split * half); c < x.columns && needed; c += 4 * split) {
+                    float v[2] = {0.0f, 0.0f};
+                    for (int r = 0; r < split; ++r) {
+                        const float* const theirs = cluster_address(left, r);
+                        v[0] += theirs[c * kTileRows + own];
+                        v[1] += theirs[(c + 1) * kTileRows + own];
+                    }
+                    finish(c, v);
+                }
+            } else if (needed) {
+                const bool spread = all_tokens(x);
+                for (int c0 = 16 * half; c0 < x.columns; c0 += 32) {
+                    float v[16];
+                    if (spread) tmem_load_spread(sums, [&](int j) { return s.list[buffer][min(c0 + j, x.columns - 1)] / p.topk; }, v);
+                    else tmem_load_16(sums + c0, v);
+                    finish(c0, v);
                 }
             }
             tcgen05_before_sync();
             __syncwarp();
-            if (lane == 0) barrier_arrive(&s.sums_empty[buffer]);
+            if (lane == 0) barrier_arrive(sums_empty0 + 8 * buffer);
             if (kOp == kLayerDown) {
                 // The tile that brings a token's last row adds its rows up, in the order of the token's choices whichever tile it is.
                 __threadfence();
-                named_sync(1, 128);
-                for (int c = at; c < x.columns; c += 128) {
-                    const int token = s.list[buffer][c] / p.topk;
+                named_sync(1, kFinishers);
+                if (at < x.columns) {
+                    const int token = s.list[buffer][at] / p.topk;
                     int due = 0;
                     for (int k = 0; k < p.topk; ++k) {
                         const int e = p.indices[token * p.topk + k];
@@ -419,17 +569,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     if (atomicAdd(&p.tickets[token * feature_tiles + x.m], 1) == due - 1) s.last[atomicAdd(&s.last_count, 1)] = token;
                 }
                 __threadfence();
-                named_sync(1, 128);
+                named_sync(1, kFinishers);
                 const int ready = s.last_count;
-                for (int i = quarter; i < ready; i += 4) {
-                    const int token = s.last[i], g = x.m * kTileRows + 4 * lane;
-                    if (g >= p.features) continue;  // features are a multiple of 8
+                for (int i = warp - 4; i < ready; i += kFinishers / 32) {
+                    const int token = s.last[i], g = x.m * height + 4 * lane;
+                    if (4 * lane >= height || g >= p.features) continue;  // both are multiples of 8
                     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     for (int k = 0; k < p.topk; ++k) {
                         const int e = p.indices[token * p.topk + k];
                         if (e < 0 || e >= p.groups) continue;
-                        const float4 part = __ldcg(reinterpret_cast<const float4*>(p.parts + ((size_t)token * p.topk + k) * p.features + g));
-                        sum.x += part.x, sum.y += part.y, sum.z += part.z, sum.w += part.w;
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.parts + ((size_t)token * p.topk + k) * p.features + g));
+                        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
                     }
                     const float out[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
@@ -439,24 +589,30 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                         static_cast<T*>(p.y)[o] = Element<T>::from_float(out[j] + r);
                     }
                 }
-                named_sync(1, 128);
+                named_sync(1, kFinishers);
                 if (at == 0) s.last_count = 0;
                 // the next tile's first named_sync orders this before its counting
             }
             if (kGrouped) {
-                if (kOp != kLayerDown) named_sync(1, 128);
-                if (at == 0) barrier_arrive(&s.list_empty[buffer]);
+                if (kOp != kLayerDown) named_sync(1, kFinishers);
+                if (at == 0) barrier_arrive(list_empty0 + 8 * buffer);
             }
         }
+        if (!met) cluster_sync();  // it gave up; the cluster's other blocks are waiting
     }
     __syncwarp();
+    // What the epilogue's threads meet at, the others meet here: nobody leaves while its sums are read.
+    if (kOp == kDense && split > 1) {
+        if (warp < 4) cluster_sync();
+        cluster_sync();
+    }
     tcgen05_before_sync();
     __syncthreads();
     tcgen05_after_sync();
     if (s.gave_up) {
         // copies and products in flight end in less than this
-        const long long begin = now_ns();
-        while (now_ns() - begin < 1000000) __nanosleep(1000);
+        const long long begin = clock64();
+        while (clock64() - begin < 2000000) __nanosleep(1000);
         if (tid == 0) atomicExch(&g_product_error, A2A_ERR_TIMEOUT);
         __syncthreads();
     }
