@@ -87,27 +87,30 @@ int opt_in() {
 }
 
 // A launch that may get ready while the one before it in the stream ends (its kernel waits for that one itself), in clusters of `cluster` blocks.
-template <TilesOp kOp, typename T>
-int launch_tiles(const TilesParams& p, int grid, int cluster, cudaStream_t st) {
-    const void* fn = reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T>);
-    const int rc = opt_in<kOp, T>();
-    if (rc != A2A_OK) return rc;
+int launch(const void* fn, dim3 grid, int threads, size_t shared, int cluster, void* params, cudaStream_t st) {
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = cluster;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t launch{};
-    launch.gridDim = dim3(grid);
-    launch.blockDim = dim3(kTilesThreads);
-    launch.dynamicSmemBytes = kTilesSharedBytes;
-    launch.stream = st;
-    launch.attrs = attr;
-    launch.numAttrs = cluster > 1 ? 2 : 1;
-    void* args[] = {const_cast<TilesParams*>(&p)};
-    const cudaError_t e = cudaLaunchKernelExC(&launch, fn, args);
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = st;
+    config.attrs = attr;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    void* args[] = {params};
+    const cudaError_t e = cudaLaunchKernelExC(&config, fn, args);
     return e == cudaSuccess ? A2A_OK : -(int)e;
+}
+
+template <TilesOp kOp, typename T>
+int launch_tiles(const TilesParams& p, int grid, int cluster, cudaStream_t st) {
+    const int rc = opt_in<kOp, T>();
+    if (rc != A2A_OK) return rc;
+    return launch(reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T>), grid, kTilesThreads, kTilesSharedBytes, cluster, const_cast<TilesParams*>(&p), st);
 }
 
 // Features of a tile and blocks that share its inner length, for a dense product: what the fullest SM needs least time for. The columns are
@@ -151,7 +154,7 @@ DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
             // all clusters run at once (they do not come to lie on every SM), or there is nothing to gain
             if (split > 1 && tiles > most_clusters<T>(split)) break;
             const int busy = std::min(tiles * split, sms), rounds = split > 1 ? 1 : parts_of(tiles, sms);
-            const float memory = busy / (6500.0f * across), t = rounds * parts_of(blocks, split) * (block_ns(paired ? 2 * height : height, columns, memory) + 15.0f) + (split > 1 ? 1500.0f : 0.0f);
+            const float memory = busy / (6500.0f * across), t = rounds * parts_of(blocks, split) * block_ns(paired ? 2 * height : height, columns, memory) + (split > 1 ? 1500.0f : 0.0f);
             if (t < least * 0.999f) least = t, best = DensePlan{height, columns, split};
         }
     return best;
@@ -177,16 +180,15 @@ int linear_of(const a2a_linear_args& a, int sms, cudaStream_t st) {
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// The workspace of a layer: the experts' inner values, the rows of every pair and the tickets.
+// The workspace of a layer: the experts' inner values, and the rows of every pair.
 struct LayerSpace {
-    size_t parts, tickets, end;
+    size_t parts, end;
 };
 LayerSpace layer_space(int tokens, int topk, int hidden_dim, int inner) {
     LayerSpace s{};
     const size_t pairs = (size_t)tokens * topk;
     s.parts = round256(pairs * inner * 2);
-    s.tickets = s.parts + round256(pairs * hidden_dim * 4);
-    s.end = s.tickets + round256((size_t)tokens * parts_of(hidden_dim, kLeastHeight) * 4);
+    s.end = s.parts + round256(pairs * hidden_dim * 4);
     return s;
 }
 
@@ -204,7 +206,8 @@ int expert_maps(TilesParams& p, int dtype, const void* weights, int experts, int
 }
 // Rows that lie in runs.
 int run_maps(TilesParams& p, int dtype, const void* rows, long long count) {
-    const int rc = rows_map(&p.rows, dtype, rows, count, p.inner, p.inner, 64);
+    int rc = rows_map(&p.rows, dtype, rows, count, p.inner, p.inner, 64);
+    if (rc == A2A_OK) rc = rows_map(&p.rows_some, dtype, rows, count, p.inner, p.inner, 32);
     return rc == A2A_OK ? rows_map(&p.rows_few, dtype, rows, count, p.inner, p.inner, 8) : rc;
 }
 
@@ -214,18 +217,25 @@ int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
     const LayerSpace at = layer_space(a.tokens, a.topk, a.hidden_dim, a.inner);
     TilesParams p{};
     p.groups = a.experts, p.tokens = a.tokens, p.topk = a.topk, p.indices = a.topk_idx, p.weights_of = a.topk_weights;
-    p.hidden = space, p.parts = reinterpret_cast<float*>(space + at.parts), p.tickets = reinterpret_cast<int*>(space + at.tickets);
-    p.ticket_count = a.tokens * parts_of(a.hidden_dim, kLeastHeight);
+    p.hidden = space, p.parts = reinterpret_cast<float*>(space + at.parts);
     p.columns = kMaxColumns;
     int rc = expert_maps(p, a.dtype, a.gate_up, a.experts, a.inner, true, a.hidden_dim);
-    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.hidden_dim, a.hidden_dim, round16(a.tokens));
-    if (rc == A2A_OK) rc = rows_map(&p.rows_few, a.dtype, a.x, a.tokens, a.hidden_dim, a.hidden_dim, 1);
+    p.sorted = a.tokens > kSpreadTokens;
+    if (rc == A2A_OK && !p.sorted) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.hidden_dim, a.hidden_dim, round16(a.tokens));
+    if (rc == A2A_OK && p.sorted) {
+        // where the second product will have its rows of pairs, which are wider
+        rc = run_maps(p, a.dtype, p.parts, (long long)a.tokens * a.topk);
+        SortParams sort{a.x, a.topk_idx, p.parts, a.tokens, a.topk, a.experts, a.hidden_dim * 2};
+        if (rc == A2A_OK) rc = launch(reinterpret_cast<const void*>(&layer_rows_kernel), parts_of(a.tokens * a.topk, kSortThreads / 32), kSortThreads, 0, 1, &sort, st);
+    }
     if (rc == A2A_OK) rc = launch_tiles<kLayerUp, T>(p, sms, 1, st);
     if (rc != A2A_OK) return rc;
-    p.residual = a.residual, p.y = a.y;
     rc = expert_maps(p, a.dtype, a.down, a.experts, a.hidden_dim, false, a.inner);
     if (rc == A2A_OK) rc = run_maps(p, a.dtype, p.hidden, (long long)a.tokens * a.topk);
-    return rc == A2A_OK ? launch_tiles<kLayerDown, T>(p, sms, 1, st) : rc;
+    if (rc == A2A_OK) rc = launch_tiles<kLayerDown, T>(p, sms, 1, st);
+    if (rc != A2A_OK) return rc;
+    SumParams sum{p.parts, a.topk_idx, a.residual, a.y, a.topk, a.experts, a.hidden_dim};
+    return launch(reinterpret_cast<const void*>(&layer_sum_kernel<T>), dim3(a.tokens, parts_of(a.hidden_dim, 4 * kSumThreads)), kSumThreads, 0, 1, &sum, st);
 }
 
 template <typename T>
