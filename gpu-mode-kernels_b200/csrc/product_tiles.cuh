@@ -7,8 +7,8 @@
 // Sums are fp32 in tensor memory, two buffers of 256 columns, so that one tile's epilogue runs beside the next one's products.
 //
 // Few rows leave the weights' bytes as the only cost, and then the SMs should have the same number of them: a tile has as many
-// features as makes the number of tiles fill the SMs (`height`), up to what 128 rows hold. Operand rows behind them are whatever lies
-// there; their sums are not read. A dense product with too few features for all SMs is cut along the inner length too, over the blocks
+// features as makes the number of tiles fill the SMs (`height`), up to what 128 rows hold, and over experts the tiles of a last round that
+// fills no SMs are cut smaller. Operand rows behind a tile's features are whatever lies there; their sums are not read. A dense product with too few features for all SMs is cut along the inner length too, over the blocks
 // of a cluster, which add up their sums in the order of their ranks through distributed shared memory.
 //
 // Where rows of x come from: dense, and in the first product of a layer of up to kSpreadTokens, a box of all rows; of such a layer an expert's
@@ -102,12 +102,29 @@ constexpr size_t kTilesSharedBytes = 1024 + kRingBytes + sizeof(TilesShared);
 static_assert(kTilesSharedBytes <= 227 * 1024, "a block's shared memory");
 
 struct Tile {
-    int group, m, first, columns;  // matrix, tile of its features, first column, columns
+    int group, f, height, first, columns;  // matrix, first feature, features, first column, columns
 };
 
-__host__ __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
 __host__ __device__ __forceinline__ int parts_of(int n, int size) { return (n + size - 1) / size; }
 
+// How `tiles` tiles of `height` features go over `blocks` blocks: whole rounds, and those of the last round in `cut` parts of `part` features.
+struct Rounds {
+    int whole, cut, part;
+};
+__host__ __device__ __forceinline__ Rounds rounds_of(int tiles, int blocks, int height, int least, int step) {
+    Rounds r;
+    r.whole = tiles / blocks;
+    const int rest = tiles - r.whole * blocks;
+    r.cut = rest > 0 ? max(1, min(blocks / rest, height / least)) : 1;
+    r.part = height;
+    if (r.cut > 1) {
+        r.part = (parts_of(height, r.cut) + step - 1) & -step;  // step: a power of two
+        r.cut = parts_of(height, r.part);
+    }
+    return r;
+}
+
+__host__ __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
 // What a block of 64 of a tile takes, in ns: the SM's share of the memory's rate for the weights (6.5 TB/s over 148), what the L2 gives an SM
 // (90 bytes a ns), or the products (256 columns by 64 in 512 cycles).
 __host__ __device__ __forceinline__ float block_ns(int rows, int columns, float memory_share) {
@@ -196,8 +213,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             unsigned cost = 0xffffffffu;
             if ((h >= piece && h < p.full) || lane == 31) {
                 const int wide = kOp == kLayerUp && !p.sorted ? round16(p.tokens) : columns;
-                const int rounds = parts_of(run * parts_of(p.features, h), gridDim.x);
-                cost = (unsigned)fminf(rounds * block_ns(h * (kUp ? 2 : 1), wide, 1.0f / 44) * 8.0f, 1e9f);
+                const int tiles = run * parts_of(p.features, h);
+                const Rounds r = rounds_of(tiles, gridDim.x, h, piece, kUp ? 4 : 8);
+                // (pieces have to be issued: 30 ns)
+                float ns = r.whole * (block_ns(h * (kUp ? 2 : 1), wide, 1.0f / 44) + (h < p.full ? 30.0f : 0.0f));
+                if (r.whole * (int)gridDim.x < tiles) ns += block_ns(r.part * (kUp ? 2 : 1), wide, 1.0f / 44) + (r.part < p.full ? 30.0f : 0.0f);
+                cost = (unsigned)fminf(ns * 8.0f, 1e9f);
             }
             const unsigned least = __reduce_min_sync(0xffffffffu, cost);
             const int best = 31 - __clz(__ballot_sync(0xffffffffu, cost == least));  // the highest of the best
@@ -213,11 +234,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                    list_full0 = shared_addr(s.list_full), list_empty0 = shared_addr(s.list_empty), ring0 = shared_addr(ring);
     const int feature_tiles = parts_of(p.features, height);
     const int across_all = kGrouped ? s.begin[p.groups] : parts_of(p.tokens, columns);
-    const int tiles = across_all * feature_tiles;
+    // over experts: the tiles that come in whole rounds, and the others in parts
+    const int piece = kPieceRows / (paired ? 2 : 1);
+    const Rounds rounds = kGrouped ? rounds_of(across_all * feature_tiles, gridDim.x, height, piece, paired ? 4 : 8) : Rounds{0, 1, height};
+    const int whole_tiles = kGrouped ? rounds.whole * gridDim.x : 0;
+    const int tiles = whole_tiles + (across_all * feature_tiles - whole_tiles) * rounds.cut;
     // the operand's columns in a stage
     const int wide = kOp == kLayerUp && !p.sorted ? round16(p.tokens) : columns;
-    const int operand_rows = paired ? 2 * height : height;
-    const int weight_bytes = (operand_rows * kRowBytes + 1023) & ~1023, block_bytes = weight_bytes + wide * kRowBytes;
+    const int highest = whole_tiles > 0 ? height : rounds.part;
+    const int weight_bytes = ((paired ? 2 : 1) * max(highest, kGrouped ? piece : 0) * kRowBytes + 1023) & ~1023, block_bytes = weight_bytes + wide * kRowBytes;
     const int blocks_all = parts_of(p.inner, kTileInner);
     const int per_stage = min(blocks_all, max(1, (kStageBytes + block_bytes / 2) / block_bytes));
     const int stages = min(kMaxStages, kRingBytes / (block_bytes * per_stage));
@@ -230,7 +255,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     // Tiles that share weights come one after the other, so that blocks read them together.
     auto tile_of = [&](int t) {
         Tile x;
-        int count;
+        int count, cut = 0;
+        x.height = height;
+        if (t >= whole_tiles && rounds.cut > 1) {
+            const int q = (t - whole_tiles) / rounds.cut;
+            cut = (t - whole_tiles - q * rounds.cut) * rounds.part;
+            t = whole_tiles + q;
+            x.height = min(rounds.part, height - cut);
+        }
         if (kGrouped) {
             const int q = t / feature_tiles;
             int lo = 0, hi = p.groups - 1;  // the last group that begins at or before q; groups without rows begin with the next
@@ -247,8 +279,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             count = p.tokens;
         }
         const int across = parts_of(count, columns);
-        x.m = t / across;
-        x.first = (t - x.m * across) * columns;
+        const int m = t / across;
+        x.f = m * height + cut;
+        x.first = (t - m * across) * columns;
         x.columns = min(columns, count - x.first);
         return x;
     };
@@ -264,12 +297,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         if (elect_one()) {
             int stage = 0;
             uint32_t phase = 1;
-            const bool whole = !kGrouped || height == p.full;  // a box of all features, or pieces
-            const int piece = kPieceRows / (paired ? 2 : 1);
-            const int bytes = whole ? operand_rows * kRowBytes : parts_of(height, piece) * kPieceRows * kRowBytes;
             for (int t = tile0; t < tiles; t += tile_step) {
                 const Tile x = tile_of(t);
-                const int f = x.m * height;
+                const int f = x.f, h1 = x.height;
+                const bool whole = !kGrouped || h1 == p.full;  // a box of all features, or pieces
+                const int bytes = whole ? (paired ? 2 : 1) * h1 * kRowBytes : parts_of(h1, piece) * kPieceRows * kRowBytes;
                 int k = block0 * kTileInner;
                 for (int left = blocks; left > 0; left -= per_stage) {
                     const uint32_t bar = full0 + 8 * stage;
@@ -281,8 +313,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                         if (whole) {
                             copy_tile_4d(at, &p.weights, k, 0, f, x.group, bar);
                         } else {
-                            for (int h0 = 0; h0 < height; h0 += piece) {
-                                const int h = min(h0, height - piece);  // the last one overlaps: the same bytes to the same place
+                            for (int h0 = 0; h0 < h1; h0 += piece) {
+                                const int h = max(0, min(h0, h1 - piece));  // the last one overlaps: the same bytes to the same place
                                 copy_tile_4d(at + h * (paired ? 2 : 1) * kRowBytes, &p.weights_piece, k, 0, f + h, x.group, bar);
                             }
                         }
@@ -458,9 +490,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             tcgen05_after_sync();
             const uint32_t sums = tmem + buffer * kMaxColumns + ((uint32_t)(quarter * 32) << 16);
             // this lane's feature
-            const int own = quarter * 32 + lane, within = paired ? own >> 1 : own, f = x.m * height + within;
-            const bool inside = within < height && f < p.features, up = paired && (lane & 1);
-            const bool needed = (paired ? quarter * 16 : quarter * 32) < height;  // by warp
+            const int own = quarter * 32 + lane, within = paired ? own >> 1 : own, f = x.f + within;
+            const bool inside = within < x.height && f < p.features, up = paired && (lane & 1);
+            const bool needed = (paired ? quarter * 16 : quarter * 32) < x.height;  // by warp
             float bias = 0.0f;
             if (kOp == kDense && p.bias != nullptr && inside)
                 bias = load_any<T>(p.bias, (size_t)(up ? p.features : 0) + f, p.bias_fp32);
