@@ -177,6 +177,8 @@ class Interpreted:
     def histogram(*_):
         return None
 
+    gate = linear = layer = histogram
+
 
 def host():
     """The compiled part of this layer (csrc/host.cpp), loaded once, or its stand-in."""

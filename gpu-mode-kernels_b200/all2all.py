@@ -18,7 +18,7 @@ from typing import Dict, Optional, Sequence, Tuple
 import torch
 import torch.distributed as dist
 
-from . import _lib
+from . import _lib, moe
 from ._lib import A2AError, Config, Status  # noqa: F401
 from .task import MoEConfig, input_t, output_t
 
@@ -48,6 +48,7 @@ class A2AContext:
             chunks = int(os.environ.get("A2A_CHUNKS", "1")) if schedule == "phased" else 1
         self.cfg, self.rank, self.world_size = cfg, rank, world_size
         self.payload, self.schedule, self.combine_mode = payload, schedule, combine
+        self._chunked = chunks > 1
         if device is None:
             device = torch.cuda.current_device() if torch.cuda.is_available() else 0
         self.device_index = int(device)
@@ -140,6 +141,17 @@ class A2AContext:
 
     def expert_done(self) -> None:
         _lib.check(self.lib.a2a_expert_done(self._h, self._stream()))
+
+    def experts(self, gate_up: torch.Tensor, down: torch.Tensor) -> None:
+        """This rank's experts (``moe.expert_mlp``) on the rows that ``dispatch_recv`` left, in place, then ``expert_done``: the
+        real expert op in the place of ``expert_placeholder``.  ``gate_up`` is ``[local experts, 2 * inner, hidden]``, ``down``
+        ``[local experts, hidden, inner]``, in the type of the rows, on this rank's GPU."""
+        if self.schedule != "phased" or self._chunked:
+            raise A2AError(_lib.A2A_ERR_STATE, "experts run between the phases of the phased schedule, of calls in one chunk")
+        with torch.cuda.device(self.device_index):
+            rows, counts = self.expert_buffers()
+            moe.expert_mlp(rows, counts, gate_up, down)
+            self.expert_done()
 
     def combine(self, weights: torch.Tensor, y: Optional[torch.Tensor] = None) -> torch.Tensor:
         assert weights.dtype == torch.float32 and weights.is_contiguous() and weights.is_cuda

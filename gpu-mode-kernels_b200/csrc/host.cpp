@@ -219,6 +219,176 @@ PyObject* histogram(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- the layer around the all-to-all ------------------------------------------------------------------
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, int device) {
+    const at::TensorOptions options = at::TensorOptions().dtype(dtype).device(at::kCUDA, (c10::DeviceIndex)device);
+    const bool heard = c10::impl::dispatch_mode_enabled() || at::hasCallbacks();
+    return heard ? at::empty(sizes, options) : at::cuda::empty(sizes, options);
+}
+
+bool sixteen(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+int32_t dtype_of(at::ScalarType t) { return t == at::kBFloat16 ? (int)A2A_DTYPE_BF16 : t == at::kHalf ? (int)A2A_DTYPE_FP16 : (int)A2A_DTYPE_FP32; }
+
+// A CUDA tensor on the current device, by its type; nullptr where it is none.
+const at::Tensor* here(PyObject* o, int* device) {
+    if (!THPVariable_CheckExact(o) || !THPVariable_Unpack(o).is_cuda()) return nullptr;
+    *device = c10::cuda::current_device();
+    return plain(o, THPVariable_Unpack(o).scalar_type(), *device);
+}
+
+// What a call answered: its output, None where the Python code is to say what is wrong, or a status code.
+PyObject* answer(int rc, at::Tensor&& out) {
+    if (rc == A2A_ERR_CONFIG) Py_RETURN_NONE;
+    if (rc != A2A_OK) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(std::move(out));
+}
+
+// gate(logits, k, score, bias, renormalize, scale): indices and weights, a status code (int) or None.
+PyObject* gate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 6) {
+        PyErr_SetString(PyExc_TypeError, "gate takes logits, k, score, bias, renormalize and scale");
+        return nullptr;
+    }
+    HANDLE_TH_ERRORS
+    int device;
+    const at::Tensor* logits = here(args[0], &device);
+    if (logits == nullptr || logits->dim() != 2 || logits->size(0) > INT32_MAX || !PyLong_CheckExact(args[1]) || !PyUnicode_CheckExact(args[2]) || !PyBool_Check(args[4]) ||
+        !PyFloat_CheckExact(args[5]))
+        Py_RETURN_NONE;
+    if (!sixteen(logits->scalar_type()) && logits->scalar_type() != at::kFloat) Py_RETURN_NONE;
+    const at::Tensor* bias = args[3] == Py_None ? nullptr : plain(args[3], at::kFloat, device);
+    if (args[3] != Py_None && (bias == nullptr || bias->dim() != 1 || bias->size(0) != logits->size(1))) Py_RETURN_NONE;
+    const long k = PyLong_AsLong(args[1]);
+    if (k == -1 && PyErr_Occurred()) PyErr_Clear();
+    const int64_t tokens = logits->size(0), experts = logits->size(1);
+    if (k < 1 || k > A2A_MAX_TOPK || k > experts || experts > A2A_MAX_EXPERTS) Py_RETURN_NONE;
+    a2a_gate_args a{};
+    if (PyUnicode_CompareWithASCIIString(args[2], "softmax") == 0) a.score = A2A_SCORE_SOFTMAX;
+    else if (PyUnicode_CompareWithASCIIString(args[2], "sigmoid") == 0) a.score = A2A_SCORE_SIGMOID;
+    else Py_RETURN_NONE;
+    at::Tensor indices = new_tensor({tokens, k}, at::kInt, device), weights = new_tensor({tokens, k}, at::kFloat, device);
+    a.logits = logits->const_data_ptr(), a.stride = experts;
+    a.bias = bias == nullptr ? nullptr : static_cast<const float*>(bias->const_data_ptr());
+    a.indices = static_cast<int32_t*>(indices.mutable_data_ptr()), a.weights = static_cast<float*>(weights.mutable_data_ptr());
+    a.tokens = (int32_t)tokens, a.experts = (int32_t)experts, a.topk = (int32_t)k, a.dtype = dtype_of(logits->scalar_type());
+    a.renormalize = args[4] == Py_True, a.scale = (float)PyFloat_AS_DOUBLE(args[5]);
+    void* stream = c10::cuda::getCurrentCUDAStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = a2a_gate(&a, stream);
+    Py_END_ALLOW_THREADS
+    if (rc == A2A_ERR_CONFIG) Py_RETURN_NONE;
+    if (rc != A2A_OK) return PyLong_FromLong(rc);
+    Ref i, w;
+    if ((i.o = THPVariable_Wrap(std::move(indices))) == nullptr || (w.o = THPVariable_Wrap(std::move(weights))) == nullptr) return nullptr;
+    return PyTuple_Pack(2, i.o, w.o);
+    END_HANDLE_TH_ERRORS
+}
+
+// linear(x, weight, bias, activation, residual, out_dtype): the output, a status code (int) or None.
+PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 6) {
+        PyErr_SetString(PyExc_TypeError, "linear takes x, weight, bias, activation, residual and a type");
+        return nullptr;
+    }
+    HANDLE_TH_ERRORS
+    int device;
+    const at::Tensor* x = here(args[0], &device);
+    if (x == nullptr || x->dim() != 2 || !sixteen(x->scalar_type()) || x->size(0) > INT32_MAX || !PyUnicode_CheckExact(args[3])) Py_RETURN_NONE;
+    const at::ScalarType dtype = x->scalar_type();
+    const int64_t tokens = x->size(0), inputs = x->size(1);
+    const at::Tensor* weight = matrix(args[1], dtype, device, -1, inputs);
+    if (weight == nullptr || inputs > A2A_MAX_PRODUCT || weight->size(0) > 2 * A2A_MAX_PRODUCT) Py_RETURN_NONE;
+    const char* const names[] = {"none", "relu", "gelu", "silu", "swiglu"};
+    a2a_linear_args a{};
+    for (a.activation = 0; a.activation <= A2A_ACT_SWIGLU; ++a.activation)
+        if (PyUnicode_CompareWithASCIIString(args[3], names[a.activation]) == 0) break;
+    const int64_t rows = weight->size(0);
+    if (a.activation > A2A_ACT_SWIGLU || (a.activation == A2A_ACT_SWIGLU && rows % 2 != 0)) Py_RETURN_NONE;
+    const int64_t outputs = a.activation == A2A_ACT_SWIGLU ? rows / 2 : rows;
+    at::ScalarType out_dtype = dtype;
+    if (args[5] != Py_None) {
+        if (!THPDtype_Check(args[5])) Py_RETURN_NONE;
+        out_dtype = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
+        if (out_dtype != dtype && out_dtype != at::kFloat) Py_RETURN_NONE;
+    }
+    a.dtype = a.bias_dtype = dtype_of(dtype), a.out_dtype = dtype_of(out_dtype);
+    if (args[2] != Py_None) {
+        const at::Tensor* bias = here(args[2], &device);
+        if (bias == nullptr || bias->dim() != 1 || bias->size(0) != rows || (bias->scalar_type() != dtype && bias->scalar_type() != at::kFloat)) Py_RETURN_NONE;
+        a.bias = bias->const_data_ptr(), a.bias_dtype = dtype_of(bias->scalar_type());
+    }
+    if (args[4] != Py_None) {
+        const at::Tensor* residual = matrix(args[4], out_dtype, device, tokens, outputs);
+        if (residual == nullptr) Py_RETURN_NONE;
+        a.residual = residual->const_data_ptr(), a.residual_stride = outputs;
+    }
+    if (outputs < 1) Py_RETURN_NONE;
+    at::Tensor y = new_tensor({tokens, outputs}, out_dtype, device);
+    a.x = x->const_data_ptr(), a.weight = weight->const_data_ptr(), a.y = y.mutable_data_ptr();
+    a.x_stride = a.weight_stride = inputs, a.y_stride = outputs;
+    a.tokens = (int32_t)tokens, a.inputs = (int32_t)inputs, a.outputs = (int32_t)outputs;
+    void* stream = c10::cuda::getCurrentCUDAStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = a2a_linear(&a, stream);
+    Py_END_ALLOW_THREADS
+    return answer(rc, std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// The weights of `experts` experts of a call on rows of `hidden` values; their inner size, or 0 where they are not plain.
+int64_t experts_of(PyObject* gate_up, PyObject* down, at::ScalarType dtype, int device, int64_t hidden, const void** up_at, const void** down_at, int64_t* experts) {
+    const at::Tensor *u = plain(gate_up, dtype, device), *d = plain(down, dtype, device);
+    if (u == nullptr || d == nullptr || u->dim() != 3 || d->dim() != 3) return 0;
+    const int64_t inner = d->size(2);
+    if (d->size(0) != u->size(0) || u->size(1) != 2 * inner || u->size(2) != hidden || d->size(1) != hidden || inner > A2A_MAX_PRODUCT ||
+        hidden > A2A_MAX_PRODUCT || d->size(0) > A2A_MAX_EXPERTS)
+        return 0;
+    *up_at = u->const_data_ptr(), *down_at = d->const_data_ptr(), *experts = d->size(0);
+    return inner;
+}
+
+// layer(x, indices, weights, gate_up, down, residual): the output, a status code (int) or None.
+PyObject* layer(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 6) {
+        PyErr_SetString(PyExc_TypeError, "layer takes x, indices, weights, gate_up, down and residual");
+        return nullptr;
+    }
+    HANDLE_TH_ERRORS
+    int device;
+    const at::Tensor* x = here(args[0], &device);
+    if (x == nullptr || x->dim() != 2 || !sixteen(x->scalar_type()) || x->size(0) < 1 || x->size(0) > A2A_MAX_LAYER_TOKENS) Py_RETURN_NONE;
+    const at::ScalarType dtype = x->scalar_type();
+    const int64_t tokens = x->size(0), hidden = x->size(1);
+    const at::Tensor* idx = plain(args[1], at::kInt, device);
+    if (idx == nullptr || idx->dim() != 2 || idx->size(0) != tokens || idx->size(1) < 1 || idx->size(1) > A2A_MAX_TOPK) Py_RETURN_NONE;
+    const int64_t topk = idx->size(1);
+    const at::Tensor* w = matrix(args[2], at::kFloat, device, tokens, topk);
+    if (w == nullptr) Py_RETURN_NONE;
+    a2a_layer_args a{};
+    int64_t experts = 0;
+    const int64_t inner = experts_of(args[3], args[4], dtype, device, hidden, &a.gate_up, &a.down, &experts);
+    if (inner == 0) Py_RETURN_NONE;
+    if (args[5] != Py_None) {
+        const at::Tensor* residual = matrix(args[5], dtype, device, tokens, hidden);
+        if (residual == nullptr) Py_RETURN_NONE;
+        a.residual = residual->const_data_ptr();
+    }
+    a.tokens = (int32_t)tokens, a.topk = (int32_t)topk, a.experts = (int32_t)experts, a.hidden_dim = (int32_t)hidden, a.inner = (int32_t)inner, a.dtype = dtype_of(dtype);
+    a.workspace_bytes = a2a_layer_workspace(a.tokens, a.topk, a.hidden_dim, a.inner);
+    at::Tensor y = new_tensor({tokens, hidden}, dtype, device), space = new_tensor({(int64_t)a.workspace_bytes}, at::kByte, device);
+    a.x = x->const_data_ptr(), a.topk_idx = static_cast<const int32_t*>(idx->const_data_ptr());
+    a.topk_weights = static_cast<const float*>(w->const_data_ptr()), a.y = y.mutable_data_ptr(), a.workspace = space.mutable_data_ptr();
+    void* stream = c10::cuda::getCurrentCUDAStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = a2a_layer(&a, stream);
+    Py_END_ALLOW_THREADS
+    return answer(rc, std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef rank_methods[] = {
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rank_forward)), METH_FASTCALL, nullptr},
     {"close", rank_close, METH_NOARGS, nullptr},
@@ -235,6 +405,9 @@ PyType_Spec rank_spec = {"_host.Rank", sizeof(Rank), 0, Py_TPFLAGS_DEFAULT, rank
 
 PyMethodDef module_methods[] = {
     {"group_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(group_forward)), METH_FASTCALL, nullptr},
+    {"gate", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gate)), METH_FASTCALL, nullptr},
+    {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear)), METH_FASTCALL, nullptr},
+    {"layer", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(layer)), METH_FASTCALL, nullptr},
     {"histogram", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(histogram)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

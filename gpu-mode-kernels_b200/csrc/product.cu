@@ -148,15 +148,19 @@ DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
     const int columns = std::min(kMaxColumns, round16(parts_of(a.tokens, across))), blocks = parts_of(a.inputs, kTileInner);
     DensePlan best{most, columns, 1};
     float least = 1e30f;
-    for (int split = 1; split <= std::min(kMaxSplit, blocks); ++split)
-        for (int height = most; height >= std::min(most, 8); --height) {
-            const int tiles = parts_of(a.outputs, height) * across;
-            // all clusters run at once (they do not come to lie on every SM), or there is nothing to gain
-            if (split > 1 && tiles > most_clusters<T>(split)) break;
+    for (int split = 1; split <= std::min(kMaxSplit, blocks); ++split) {
+        // all clusters run at once (they do not come to lie on every SM), or there is nothing to gain; whole blocks go twice over the SMs
+        // at most, or are whole tiles
+        const int room = split > 1 ? most_clusters<T>(split) : 2 * sms;
+        for (int down = parts_of(a.outputs, most); down == parts_of(a.outputs, most) || down * across <= room; ++down) {
+            const int height = parts_of(a.outputs, down), tiles = parts_of(a.outputs, height) * across;
+            if ((split > 1 && tiles > room) || (height < 8 && height < most)) break;
             const int busy = std::min(tiles * split, sms), rounds = split > 1 ? 1 : parts_of(tiles, sms);
-            const float memory = busy / (6500.0f * across), t = rounds * parts_of(blocks, split) * block_ns(paired ? 2 * height : height, columns, memory) + (split > 1 ? 1500.0f : 0.0f);
+            const float t = rounds * parts_of(blocks, split) * block_ns(paired ? 2 * height : height, columns, busy / (6500.0f * across)) +
+                            (split > 1 ? 1500.0f : 0.0f);
             if (t < least * 0.999f) least = t, best = DensePlan{height, columns, split};
         }
+    }
     return best;
 }
 

@@ -37,8 +37,13 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     further apart), ``inputs`` and the distance of rows a multiple of 8, starts on 16 bytes.  ``activation``: ``"none"``, ``"relu"``, ``"gelu"``
     (by the error function), ``"silu"``, or ``"swiglu"``: ``weight`` ``[2 * outputs, inputs]`` holds gate rows before up rows and the result is
     ``silu(gate) * up``.  ``bias`` has the weight's rows, in its type or fp32; ``residual`` the result's shape and type.  ``out_dtype``: the
-    type of ``x`` (default) or ``torch.float32``.  Sums and the epilogue are fp32, with one rounding at the end.
+    type of ``x`` (default) or ``torch.float32``.  Sums and the epilogue are fp32, with one rounding at the end.  For inference: no gradient is
+    recorded.
     """
+    out = _lib.host().linear(x, weight, bias, activation, residual, out_dtype)
+    if out is not None:
+        return out if type(out) is not int else _lib.check(out)
+    # something is wrong, or unusual: look again, one thing at a time
     if x.dtype not in _SIXTEEN or not x.is_cuda or x.dim() < 1:
         refuse(f"x must be a bf16 or fp16 CUDA tensor [..., inputs], got {x.dtype} {tuple(x.shape)} on {x.device}")
     device = x.get_device()

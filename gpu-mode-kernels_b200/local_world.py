@@ -16,7 +16,7 @@ says nothing of a group with a GPU per rank, which runs the one-launch kernel (c
 from __future__ import annotations
 
 import ctypes as C
-from typing import List, Sequence
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -83,9 +83,17 @@ class LocalWorld:
         self._send(rank_datas)
         self._step("recv")
 
-    def forward_phases(self, rank_datas: Sequence) -> List[torch.Tensor]:
+    def forward_phases(self, rank_datas: Sequence, experts: Optional[Sequence] = None) -> List[torch.Tensor]:
         """The four public phases, one after the other and handed on from one to the next: a program with expert kernels of its
-        own calls them one by one, in which each launch also raises and awaits flags."""
+        own calls them one by one, in which each launch also raises and awaits flags.  With ``experts``, a pair ``(gate_up, down)`` for
+        every rank, these run in the place of the placeholder (``A2AContext.experts``)."""
+        if experts is not None:
+            if len(experts) != self.world_size:
+                raise _lib.A2AError(_lib.A2A_ERR_STATE, f"{self.world_size} ranks, but experts for {len(experts)}")
+            self.dispatch(rank_datas)
+            for c, (gate_up, down) in zip(self.ctxs, experts):
+                c.experts(gate_up, down)
+            return self._combine(rank_datas)
         ys = self._quick(rank_datas, _PHASES, False)
         if ys is not None:
             return ys

@@ -30,7 +30,12 @@ def topk_gate(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Opt
     k largest ``score + bias`` (in 64 bits; the bias is not part of the weights), in descending order, ties to the lowest index.  Weights are the
     chosen scores, divided by their sum with ``renormalize`` (0 where that is 0), times ``scale``.  A logit of -inf excludes an expert while k
     others are there; a row of nothing else gets weights 0 with softmax.  NaN ranks first, and the weights of its row are NaN with softmax.
+    For inference: no gradient is recorded.
     """
+    out = _lib.host().gate(logits, k, score, bias, renormalize, scale)
+    if out is not None:
+        return out if type(out) is not int else _lib.check(out)
+    # something is wrong, or unusual: look again, one thing at a time
     if logits.dtype not in DTYPES or not logits.is_cuda or logits.dim() != 2:
         refuse(f"logits must be a [tokens, experts] CUDA tensor of fp32, bf16 or fp16, got {tuple(logits.shape)} {logits.dtype} on {logits.device}")
     device = logits.get_device()
@@ -88,8 +93,12 @@ def moe_layer(x: torch.Tensor, indices: torch.Tensor, weights: torch.Tensor, gat
     ``x``, the experts and ``residual`` (or None) share one type, bf16 or fp16; ``indices`` int32 and ``weights`` fp32 are ``[tokens, k]``.  An
     index outside the experts marks none (a padded token's row is its residual, or 0); the same expert twice counts twice.  Sums are fp32;
     an expert's inner values are rounded to the type, since the second product takes 16-bit operands, and the result once.
-    More tokens go through ``A2AContext`` with ``experts`` between dispatch and combine.
+    More tokens go through ``A2AContext`` with ``experts`` between dispatch and combine.  For inference: no gradient is recorded.
     """
+    out = _lib.host().layer(x, indices, weights, gate_up, down, residual)
+    if out is not None:
+        return out if type(out) is not int else _lib.check(out)
+    # something is wrong, or unusual: look again, one thing at a time
     if x.dtype not in _SIXTEEN or not x.is_cuda or x.dim() != 2 or not x.is_contiguous():
         refuse(f"x must be a contiguous bf16 or fp16 CUDA tensor [tokens, hidden], got {x.dtype} {tuple(x.shape)} on {x.device}")
     device = x.get_device()
