@@ -242,6 +242,9 @@ int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
     return launch(reinterpret_cast<const void*>(&layer_sum_kernel<T>), dim3(a.tokens, parts_of(a.hidden_dim, 4 * kSumThreads)), kSumThreads, 0, 1, &sum, st);
 }
 
+// Rows of inner values that a call on slabs may have: those of a slab are rounded up to whole boxes of eight.
+long long inner_rows(int local_experts, int world, int capacity) { return (long long)local_experts * world * ((capacity + 7) & ~7); }
+
 template <typename T>
 int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {
     const long long rows = (long long)a.local_experts * a.world * a.capacity;
@@ -254,7 +257,7 @@ int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {
     if (rc != A2A_OK) return rc;
     p.y = a.out;
     rc = expert_maps(p, a.dtype, a.down, a.local_experts, a.hidden_dim, false, a.inner);
-    if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.workspace, rows);
+    if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.workspace, inner_rows(a.local_experts, a.world, a.capacity));
     return rc == A2A_OK ? launch_tiles<kSlabDown, T>(p, sms, 1, st) : rc;
 }
 
@@ -306,7 +309,7 @@ extern "C" int a2a_layer(const a2a_layer_args* args, void* stream) {
 
 extern "C" size_t a2a_experts_workspace(int local_experts, int world_size, int capacity, int inner) {
     if (local_experts < 1 || world_size < 1 || capacity < 1 || inner < 1) return 0;
-    return round256((size_t)local_experts * world_size * capacity * inner * 2);
+    return round256((size_t)inner_rows(local_experts, world_size, capacity) * inner * 2);
 }
 
 extern "C" int a2a_experts(const a2a_experts_args* args, void* stream) {

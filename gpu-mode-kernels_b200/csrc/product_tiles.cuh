@@ -38,7 +38,9 @@ constexpr int kTileRows = 128, kTileInner = 64, kMaxColumns = 256;
 constexpr int kRowBytes = kTileInner * 2;
 constexpr int kTilesThreads = 384, kFinishers = 256;  // of which the epilogue's
 constexpr int kRingBytes = 192 * 1024, kMaxStages = 12;
-constexpr int kStageBytes = 32 * 1024;  // a stage has as many blocks of 64 as reach this, so that small tiles do not pay a barrier for each
+// A stage has about as many blocks of 64 as reach this: small tiles do not pay a barrier for each, and two blocks of a row's 128 bytes come
+// one right after the other, which the memory likes (experts on slabs of 7 rows: 221 us with 32 KB, 194 with 48, 207 with 64).
+constexpr int kStageBytes = 48 * 1024;
 constexpr int kMaxGroups = A2A_MAX_EXPERTS;
 constexpr int kTmemColumns = 512;
 constexpr int kSpreadTokens = 64;  // 40 to 100 tokens take the same either way
@@ -71,7 +73,7 @@ struct TilesParams {
     const float* weights_of;
     int topk;
     int sorted;    // kLayerUp: `rows` are the pairs' rows by expert, and a launch of the same call has put them there
-    void* hidden;  // kLayerUp: [pair, by expert][features]; kSlabUp: [row of the slabs][features]
+    void* hidden;  // kLayerUp: [pair, by expert][features]; kSlabUp: [column, by expert][features]
     float* parts;  // [pair][features] of kLayerDown
     // kSlab*
     const int* counts;
@@ -88,7 +90,7 @@ struct TilesShared {
     int height;
     int begin[kMaxGroups + 1];  // tiles of one feature tile before a group's
     int count[kMaxGroups];      // columns of a group
-    int row[kMaxGroups];        // rows before a group's (kLayer*)
+    int row[kMaxGroups];        // columns before a group's
     int list[2][kMaxColumns];   // columns of a tile: pair (kLayer*) or row of the slabs, -1 for none
     float scale[2][kMaxColumns];
     int2 box[2][kMaxColumns / 8];  // kSlab*: boxes of 64, of 32 and of 8 rows: first row and column
@@ -136,9 +138,9 @@ __host__ __device__ __forceinline__ float block_ns(int rows, int columns, float 
 template <TilesOp kOp, typename T>
 __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const __grid_constant__ TilesParams p) {
     constexpr bool kGrouped = kOp != kDense, kLayer = kOp == kLayerUp || kOp == kLayerDown, kSlab = kOp == kSlabUp || kOp == kSlabDown;
-    const bool first = kOp == kDense || (kOp == kLayerUp && !p.sorted) || kOp == kSlabUp;  // nothing of the same call runs before it
-    const bool runs = kOp == kLayerDown || (kOp == kLayerUp && p.sorted);                 // rows by expert
     constexpr bool kUp = kOp == kLayerUp || kOp == kSlabUp;
+    const bool first = kOp == kDense || (kOp == kLayerUp && !p.sorted) || kOp == kSlabUp;  // nothing of the same call runs before it
+    const bool runs = kGrouped && (!kUp || (kOp == kLayerUp && p.sorted));              // rows by expert
     extern __shared__ uint8_t shared_raw[];
     uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(shared_raw) + 1023) & ~(uintptr_t)1023);
     TilesShared& s = *reinterpret_cast<TilesShared*>(ring + kRingBytes);
@@ -154,7 +156,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             barrier_init(&s.sums_full[i], 1);
             barrier_init(&s.sums_empty[i], kFinishers / 32);
             barrier_init(&s.list_full[i], 1);
-            barrier_init(&s.list_empty[i], kLayer ? 1 : 2);  // the roles that read it
+            barrier_init(&s.list_empty[i], kOp == kSlabUp ? 2 : 1);  // the roles that read it
         }
         s.gave_up = s.largest = 0;
         barrier_init_done();
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     run = (x.columns + 7) & ~7;
                     const int size = run >= 64 ? 64 : run >= 32 ? 32 : 8;
                     bytes = (run + size - 1) / size * size * kRowBytes;
-                } else if (kSlab) {
+                } else if (kOp == kSlabUp) {
                     if (!barrier_wait(list_full0 + 8 * (n & 1), (n >> 1) & 1, &s.gave_up)) goto rows_done;
                     wide_boxes = s.boxes[n & 1][0], some_boxes = s.boxes[n & 1][1], boxes = s.boxes[n & 1][2];
                     bytes = (64 * wide_boxes + 32 * (some_boxes - wide_boxes) + 8 * (boxes - some_boxes)) * kRowBytes;
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     }
                     if (++stage == stages) stage = 0, phase ^= 1;
                 }
-                if (kSlab) barrier_arrive(list_empty0 + 8 * (n & 1));
+                if (kOp == kSlabUp) barrier_arrive(list_empty0 + 8 * (n & 1));
             }
         rows_done:;
         }
@@ -524,8 +526,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                             store_any<T>(p.y, (size_t)(x.first + c) * p.y_stride + f, out[j], p.out_fp32);
                         } else {
                             // Rounded to the rows' type, since the next product takes 16-bit operands.
-                            const int row = kOp == kLayerUp ? s.row[x.group] + x.first + c : s.list[buffer][c];
-                            if (row >= 0) static_cast<T*>(p.hidden)[(size_t)row * p.features + f] = Element<T>::from_float(out[j]);
+                            if (kOp == kLayerUp || s.list[buffer][c] >= 0)
+                                static_cast<T*>(p.hidden)[(size_t)(s.row[x.group] + x.first + c) * p.features + f] = Element<T>::from_float(out[j]);
                         }
                     }
                     return;
