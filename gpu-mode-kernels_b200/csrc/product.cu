@@ -2,6 +2,8 @@
 //
 // All of them are product_tiles.cuh's kernel.
 #include <algorithm>
+#include <cstdio>
+#include <cstdlib>
 #include <atomic>
 
 #include "product_device.cuh"
@@ -73,17 +75,44 @@ int sm_count(int* sms) {
 }
 
 // Lets the kernel have its shared memory on the current device.
-template <TilesOp kOp, typename T>
+template <TilesOp kOp, typename T, bool kPair>
 int opt_in() {
     static std::atomic<unsigned long long> opted{0};  // a bit a device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return -(int)e;
     if (dev < 64 && (opted.load(std::memory_order_acquire) >> dev & 1)) return A2A_OK;
-    e = cudaFuncSetAttribute((const void*)&product_tiles_kernel<kOp, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTilesSharedBytes);
+    e = cudaFuncSetAttribute((const void*)&product_tiles_kernel<kOp, T, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTilesSharedBytes);
     if (e != cudaSuccess) return -(int)e;
     if (dev < 64) opted.fetch_or(1ull << dev, std::memory_order_release);
     return A2A_OK;
+}
+
+// How many clusters of `size` blocks run at once: they do not come to lie on every SM.
+template <TilesOp kOp, typename T, bool kPair>
+int most_clusters(int size) {
+    static std::atomic<int> known[kMaxSplit + 1];  // one more than the number; of the first device that asked, as all are alike
+    int n = known[size].load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = size;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(size);
+        config.blockDim = dim3(kTilesThreads);
+        config.dynamicSmemBytes = kTilesSharedBytes;
+        config.attrs = &attr;
+        config.numAttrs = 1;
+        if (opt_in<kOp, T, kPair>() != A2A_OK ||
+            cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T, kPair>), &config) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        known[size].store(++n, std::memory_order_relaxed);
+        if (getenv("XP")) printf("op %d pair %d clusters of %d: %d\n", (int)kOp, (int)kPair, size, n - 1);
+    }
+    return n - 1;
 }
 
 // A launch that may get ready while the one before it in the stream ends (its kernel waits for that one itself), in clusters of `cluster` blocks.
@@ -106,61 +135,43 @@ int launch(const void* fn, dim3 grid, int threads, size_t shared, int cluster, v
     return e == cudaSuccess ? A2A_OK : -(int)e;
 }
 
-template <TilesOp kOp, typename T>
+template <TilesOp kOp, typename T, bool kPair = false>
 int launch_tiles(const TilesParams& p, int grid, int cluster, cudaStream_t st) {
-    const int rc = opt_in<kOp, T>();
+    const int rc = opt_in<kOp, T, kPair>();
     if (rc != A2A_OK) return rc;
-    return launch(reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T>), grid, kTilesThreads, kTilesSharedBytes, cluster, const_cast<TilesParams*>(&p), st);
+    return launch(reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T, kPair>), grid, kTilesThreads, kTilesSharedBytes, cluster, const_cast<TilesParams*>(&p), st);
 }
 
 // Features of a tile and blocks that share its inner length, for a dense product: what the fullest SM needs least time for. The columns are
 // as many as there are, up to 256.
 struct DensePlan {
     int height, columns, split;
+    bool pair;
 };
-template <typename T>
-int most_clusters(int size) {
-    static std::atomic<int> known[kMaxSplit + 1];  // one more than the number; of the first device that asked, as all are alike
-    int n = known[size].load(std::memory_order_relaxed);
-    if (n == 0) {
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = size;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cudaLaunchConfig_t launch{};
-        launch.gridDim = dim3(size);
-        launch.blockDim = dim3(kTilesThreads);
-        launch.dynamicSmemBytes = kTilesSharedBytes;
-        launch.attrs = &attr;
-        launch.numAttrs = 1;
-        if (opt_in<kDense, T>() != A2A_OK || cudaOccupancyMaxActiveClusters(&n, (const void*)&product_tiles_kernel<kDense, T>, &launch) != cudaSuccess) {
-            cudaGetLastError();
-            return 0;
-        }
-        known[size].store(++n, std::memory_order_relaxed);
-    }
-    return n - 1;
-}
-
 template <typename T>
 DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
     const int most = std::min(paired ? kTileRows / 2 : kTileRows, a.outputs), across = parts_of(a.tokens, kMaxColumns);
     const int columns = std::min(kMaxColumns, round16(parts_of(a.tokens, across))), blocks = parts_of(a.inputs, kTileInner);
-    DensePlan best{most, columns, 1};
+    DensePlan best{most, columns, 1, false};
     float least = 1e30f;
     for (int split = 1; split <= std::min(kMaxSplit, blocks); ++split) {
         // all clusters run at once (they do not come to lie on every SM), or there is nothing to gain; whole blocks go twice over the SMs
         // at most, or are whole tiles
-        const int room = split > 1 ? most_clusters<T>(split) : 2 * sms;
+        const int room = split > 1 ? most_clusters<kDense, T, false>(split) : 2 * sms;
         for (int down = parts_of(a.outputs, most); down == parts_of(a.outputs, most) || down * across <= room; ++down) {
             const int height = parts_of(a.outputs, down), tiles = parts_of(a.outputs, height) * across;
             if ((split > 1 && tiles > room) || (height < 8 && height < most)) break;
             const int busy = std::min(tiles * split, sms), rounds = split > 1 ? 1 : parts_of(tiles, sms);
-            const float t = rounds * parts_of(blocks, split) * block_ns(paired ? 2 * height : height, columns, busy / (6500.0f * across)) +
+            const float t = rounds * parts_of(blocks, split) * block_ns(paired ? 2 * height : height, columns, columns, busy / (6500.0f * across)) +
                             (split > 1 ? 1500.0f : 0.0f);
-            if (t < least * 0.999f) least = t, best = DensePlan{height, columns, split};
+            if (t < least * 0.999f) least = t, best = DensePlan{height, columns, split, false};
         }
     }
+    // pairs of blocks, with whole tiles
+    const int wide = std::min(kMaxColumns, (parts_of(a.tokens, across) + 31) / 32 * 32), tiles = parts_of(a.outputs, 2 * most) * across, units = most_clusters<kDense, T, true>(2);
+    if (units < 1) return best;
+    const float t = parts_of(tiles, units) * blocks * block_ns(paired ? 2 * most : most, wide, wide / 2, 2 * std::min(tiles, units) / (6500.0f * across));
+    if (t < least) best = DensePlan{most, wide, 1, true};
     return best;
 }
 
@@ -176,8 +187,12 @@ int linear_of(const a2a_linear_args& a, int sms, cudaStream_t st) {
     const DensePlan plan = dense_plan<T>(a, paired, sms);
     p.columns = plan.columns, p.full = plan.height, p.split = plan.split;
     int rc = weights_map(&p.weights, a.dtype, a.weight, 1, a.outputs, paired, a.inputs, a.weight_stride, plan.height);
-    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.inputs, a.x_stride, p.columns);
+    if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.inputs, a.x_stride, plan.pair ? p.columns / 2 : p.columns);
     if (rc != A2A_OK) return rc;
+    if (plan.pair) {
+        const int tiles = parts_of(a.outputs, 2 * plan.height) * parts_of(a.tokens, plan.columns);
+        return launch_tiles<kDense, T, true>(p, 2 * std::min(tiles, most_clusters<kDense, T, true>(2)), 2, st);
+    }
     const int tiles = parts_of(a.outputs, plan.height) * parts_of(a.tokens, plan.columns);
     return launch_tiles<kDense, T>(p, plan.split > 1 ? tiles * plan.split : std::min(tiles, sms), plan.split, st);
 }
@@ -253,12 +268,12 @@ int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {
     p.columns = kMaxColumns;
     int rc = expert_maps(p, a.dtype, a.gate_up, a.local_experts, a.inner, true, a.hidden_dim);
     if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.rows, rows);
-    if (rc == A2A_OK) rc = launch_tiles<kSlabUp, T>(p, sms, 1, st);
+    if (rc == A2A_OK) rc = launch_tiles<kSlabUp, T, true>(p, 2 * std::max(1, most_clusters<kSlabUp, T, true>(2)), 2, st);
     if (rc != A2A_OK) return rc;
     p.y = a.out;
     rc = expert_maps(p, a.dtype, a.down, a.local_experts, a.hidden_dim, false, a.inner);
     if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.workspace, inner_rows(a.local_experts, a.world, a.capacity));
-    return rc == A2A_OK ? launch_tiles<kSlabDown, T>(p, sms, 1, st) : rc;
+    return rc == A2A_OK ? launch_tiles<kSlabDown, T, true>(p, 2 * std::max(1, most_clusters<kSlabDown, T, true>(2)), 2, st) : rc;
 }
 
 bool dtype16(int dtype) { return dtype == A2A_DTYPE_BF16 || dtype == A2A_DTYPE_FP16; }

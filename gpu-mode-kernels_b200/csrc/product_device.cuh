@@ -90,6 +90,15 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
+// The same barrier of the first block of this block's cluster.
+__device__ __forceinline__ uint32_t of_first_block(uint32_t bar) {
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(bar));
+    return there;
+}
+__device__ __forceinline__ void barrier_arrive_there(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // Waits for the phase of `parity`; false where the block has given up, or does now because the time has run out.
 __device__ __noinline__ bool barrier_wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up) {
     const long long begin = clock64();
@@ -123,44 +132,77 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
+// kPair: of a pair of blocks, whose products one of them issues; its barrier is told of both blocks' copies.
+template <bool kPair>
 __device__ __forceinline__ void copy_tile_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
-                 : "memory");
+    if constexpr (kPair)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+                     : "memory");
 }
+template <bool kPair>
 __device__ __forceinline__ void copy_tile_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-        : "memory");
-}
-// Four rows anywhere in the matrix, one under the other.
-__device__ __forceinline__ void copy_rows_4(uint32_t dst, const CUtensorMap* map, int x, int r0, int r1, int r2, int r3, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
-        : "memory");
+    if constexpr (kPair)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+            : "memory");
 }
 
 // ---- tensor core (tcgen05) -------------------------------------------------------------------------
+// kPair: by the same warp of both blocks of a pair, and products of 256 rows, 128 of each block, issued by the first.
+template <bool kPair>
 __device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(where)), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (kPair) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(where)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(where)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
 }
+template <bool kPair>
 __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+    if constexpr (kPair)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+    else
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
 }
 __device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Arrives at the barrier, of both blocks of a pair, when the products so far are through.
+template <bool kPair>
 __device__ __forceinline__ void tcgen05_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if constexpr (kPair)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+template <bool kPair>
 __device__ __forceinline__ void tcgen05_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t descriptor, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(descriptor), "r"((uint32_t)add)
-        : "memory");
+    if constexpr (kPair)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(descriptor), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(descriptor), "r"((uint32_t)add)
+            : "memory");
 }
 // 16 columns of this warp's 32 lanes: a lane's values of columns c to c + 15.
 __device__ __forceinline__ void tmem_load_16(uint32_t tmem, float (&v)[16]) {
@@ -198,9 +240,9 @@ __device__ __forceinline__ uint64_t operand_descriptor(uint32_t at) {
     return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
            (uint64_t)2 << 61;
 }
-// fp32 sums of products of `format` (Element::kFormat), 128 rows by `columns`, both operands K-major.
-__device__ __forceinline__ uint32_t instruction_descriptor(unsigned format, int columns) {
-    return 1u << 4 | format << 7 | format << 10 | (uint32_t)(columns >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+// fp32 sums of products of `format` (Element::kFormat), `rows` rows by `columns`, both operands K-major.
+__device__ __forceinline__ uint32_t instruction_descriptor(unsigned format, int rows, int columns) {
+    return 1u << 4 | format << 7 | format << 10 | (uint32_t)(columns >> 3) << 17 | (uint32_t)(rows >> 4) << 24;
 }
 
 // All threads of the cluster's blocks meet; what one wrote to its shared memory before, the others see after.

@@ -24,6 +24,11 @@
 // Roles of the twelve warps: 0 weights, 1 products, 2 rows, 3 the lists of rows, 4 to 11 the epilogue, two for each 32 lanes of the tensor
 // memory: every other 16 columns each.
 //
+// Pairs of blocks (kPair): a product of 256 columns by 128 rows takes 48 KB of operands for 512 cycles, more than the L2 gives an SM (2048
+// rows of 7168, SwiGLU to 2048: 100 us). Two blocks of a cluster therefore take 256 rows between them, each with its half of the weights' rows
+// and of the columns in shared memory, 32 KB; the first block issues the products of both, and its `full` barriers expect and hear of both blocks'
+// copies. (With arrivals of the other block's producers there, a release at cluster scope a stage: 129 us.)
+//
 // SwiGLU: a tile's operand rows are gate and up of its features in turn (the tensor map's second dimension steps from gate to up), so that
 // neighbouring lanes of the epilogue hold the two and exchange by shuffles.
 #pragma once
@@ -95,6 +100,7 @@ struct TilesShared {
     float scale[2][kMaxColumns];
     int2 box[2][kMaxColumns / 8];  // kSlab*: boxes of 64, of 32 and of 8 rows: first row and column
     int boxes[2][3];               // where each kind ends
+    int box_rows[2];               // rows of all boxes, of both blocks of a pair
     short expert[kCached];         // kLayer*: expert of a pair, -1 for none
 };
 // An operand of less than 128 rows at the end of the ring is read beyond it.
@@ -128,14 +134,14 @@ __host__ __device__ __forceinline__ Rounds rounds_of(int tiles, int blocks, int 
 
 __host__ __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
 // What a block of 64 of a tile takes, in ns: the SM's share of the memory's rate for the weights (6.5 TB/s over 148), what the L2 gives an SM
-// (90 bytes a ns), or the products (256 columns by 64 in 512 cycles).
-__host__ __device__ __forceinline__ float block_ns(int rows, int columns, float memory_share) {
-    const float memory = rows * kRowBytes * memory_share, cache = (rows + columns) * kRowBytes * (1.0f / 90), products = columns * 1.05f;
+// (90 bytes a ns; `held` of the columns are this block's to copy), or the products (256 columns by 64 in 512 cycles).
+__host__ __device__ __forceinline__ float block_ns(int rows, int columns, int held, float memory_share) {
+    const float memory = rows * kRowBytes * memory_share, cache = (rows + held) * kRowBytes * (1.0f / 90), products = columns * 1.05f;
     // below 110 ns the threads that issue copies and products do not keep up
     return fmaxf(fmaxf(fmaxf(memory, cache), products), 110.0f) + 10.0f;
 }
 
-template <TilesOp kOp, typename T>
+template <TilesOp kOp, typename T, bool kPair>
 __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const __grid_constant__ TilesParams p) {
     constexpr bool kGrouped = kOp != kDense, kLayer = kOp == kLayerUp || kOp == kLayerDown, kSlab = kOp == kSlabUp || kOp == kSlabDown;
     constexpr bool kUp = kOp == kLayerUp || kOp == kSlabUp;
@@ -146,6 +152,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     TilesShared& s = *reinterpret_cast<TilesShared*>(ring + kRingBytes);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool paired = kUp || (kOp == kDense && p.paired);
+    constexpr int kBlocks = kPair ? 2 : 1, kColumnStep = 16 * kBlocks;
+    const int side = kPair ? (int)blockIdx.x & 1 : 0, units = (int)gridDim.x / kBlocks;  // block of the pair; blocks or pairs
 
     if (tid == 0) {
         for (int i = 0; i < kMaxStages; ++i) {
@@ -154,14 +162,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         }
         for (int i = 0; i < 2; ++i) {
             barrier_init(&s.sums_full[i], 1);
-            barrier_init(&s.sums_empty[i], kFinishers / 32);
+            barrier_init(&s.sums_empty[i], kFinishers / 32 * kBlocks);
             barrier_init(&s.list_full[i], 1);
             barrier_init(&s.list_empty[i], kOp == kSlabUp ? 2 : 1);  // the roles that read it
         }
         s.gave_up = s.largest = 0;
         barrier_init_done();
     }
-    if (warp == 1) tmem_alloc(&s.tmem, kTmemColumns);
+    if (warp == 1) tmem_alloc<kPair>(&s.tmem, kTmemColumns);
     if (warp == 2 && lane < (!kGrouped ? 2 : kOp == kLayerUp && !p.sorted ? 3 : 4))
         prefetch_map(lane == 0 ? &p.weights : lane == 1 ? &p.rows : lane == 2 ? &p.weights_piece : &p.rows_few);
     // A call's later launches read weights, indices and counts ahead of this: what wrote those was through before the call's first launch let
@@ -195,7 +203,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0) atomicMax(&s.largest, most);
         __syncthreads();
-        columns = min(p.columns, max(16, round16(s.largest)));
+        columns = min(p.columns, (max(s.largest, 1) + kColumnStep - 1) / kColumnStep * kColumnStep);
         if (warp == 0) {
             int run = 0, rows = 0;
             for (int g0 = 0; g0 < p.groups; g0 += 32) {
@@ -215,11 +223,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             unsigned cost = 0xffffffffu;
             if ((h >= piece && h < p.full) || lane == 31) {
                 const int wide = kOp == kLayerUp && !p.sorted ? round16(p.tokens) : columns;
-                const int tiles = run * parts_of(p.features, h);
-                const Rounds r = rounds_of(tiles, gridDim.x, h, piece, kUp ? 4 : 8);
+                const int tiles = run * parts_of(p.features, kBlocks * h);
+                const Rounds r = rounds_of(tiles, units, h, piece, kUp ? 4 : 8);
                 // (pieces have to be issued: 30 ns)
-                float ns = r.whole * (block_ns(h * (kUp ? 2 : 1), wide, 1.0f / 44) + (h < p.full ? 30.0f : 0.0f));
-                if (r.whole * (int)gridDim.x < tiles) ns += block_ns(r.part * (kUp ? 2 : 1), wide, 1.0f / 44) + (r.part < p.full ? 30.0f : 0.0f);
+                float ns = r.whole * (block_ns(h * (kUp ? 2 : 1), wide, wide / kBlocks, 1.0f / 44) + (h < p.full ? 30.0f : 0.0f));
+                if (r.whole * units < tiles) ns += block_ns(r.part * (kUp ? 2 : 1), wide, wide / kBlocks, 1.0f / 44) + (r.part < p.full ? 30.0f : 0.0f);
                 cost = (unsigned)fminf(ns * 8.0f, 1e9f);
             }
             const unsigned least = __reduce_min_sync(0xffffffffu, cost);
@@ -229,30 +237,30 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     }
     tcgen05_before_sync();
     __syncthreads();
+    if (kPair) cluster_sync();  // the other block's barriers are there
     tcgen05_after_sync();
     if (kGrouped) height = s.height;
     const uint32_t tmem = s.tmem;
     const uint32_t full0 = shared_addr(s.full), empty0 = shared_addr(s.empty), sums_full0 = shared_addr(s.sums_full), sums_empty0 = shared_addr(s.sums_empty),
                    list_full0 = shared_addr(s.list_full), list_empty0 = shared_addr(s.list_empty), ring0 = shared_addr(ring);
-    const int feature_tiles = parts_of(p.features, height);
+    const int feature_tiles = parts_of(p.features, kBlocks * height);
     const int across_all = kGrouped ? s.begin[p.groups] : parts_of(p.tokens, columns);
     // over experts: the tiles that come in whole rounds, and the others in parts
     const int piece = kPieceRows / (paired ? 2 : 1);
-    const Rounds rounds = kGrouped ? rounds_of(across_all * feature_tiles, gridDim.x, height, piece, paired ? 4 : 8) : Rounds{0, 1, height};
-    const int whole_tiles = kGrouped ? rounds.whole * gridDim.x : 0;
+    const Rounds rounds = kGrouped ? rounds_of(across_all * feature_tiles, units, height, piece, paired ? 4 : 8) : Rounds{0, 1, height};
+    const int whole_tiles = kGrouped ? rounds.whole * units : 0;
     const int tiles = whole_tiles + (across_all * feature_tiles - whole_tiles) * rounds.cut;
-    // the operand's columns in a stage
-    const int wide = kOp == kLayerUp && !p.sorted ? round16(p.tokens) : columns;
+    // the operand's columns in a stage, of this block
+    const int wide = kOp == kLayerUp && !p.sorted ? round16(p.tokens) : columns / kBlocks;
     const int highest = whole_tiles > 0 ? height : rounds.part;
     const int weight_bytes = ((paired ? 2 : 1) * max(highest, kGrouped ? piece : 0) * kRowBytes + 1023) & ~1023, block_bytes = weight_bytes + wide * kRowBytes;
     const int blocks_all = parts_of(p.inner, kTileInner);
     const int per_stage = min(blocks_all, max(1, (kStageBytes + block_bytes / 2) / block_bytes));
     const int stages = min(kMaxStages, kRingBytes / (block_bytes * per_stage));
     // this block's part of the inner length, and its tiles
-    const int split = kOp == kDense ? p.split : 1, part = kOp == kDense ? (int)blockIdx.x % split : 0;
+    const int split = kOp == kDense && !kPair ? p.split : 1, part = kOp == kDense && !kPair ? (int)blockIdx.x % split : 0;
     const int block0 = blocks_all * part / split, blocks = blocks_all * (part + 1) / split - block0;
-    const int steps = parts_of(blocks, per_stage);
-    const int tile0 = (int)blockIdx.x / split, tile_step = (int)gridDim.x / split;
+    const int tile0 = (int)blockIdx.x / (kBlocks * split), tile_step = units / split;
 
     // Tiles that share weights come one after the other, so that blocks read them together.
     auto tile_of = [&](int t) {
@@ -282,10 +290,25 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         }
         const int across = parts_of(count, columns);
         const int m = t / across;
-        x.f = m * height + cut;
+        x.f = kBlocks * (m * height + cut) + side * x.height;  // this block's
+
         x.first = (t - m * across) * columns;
         x.columns = min(columns, count - x.first);
         return x;
+    };
+    // columns of a tile's product, and of those the ones that block `of` of the pair copies
+    auto product_columns = [&](const Tile& x) {
+        if (kOp == kDense && kPair) return columns;
+        return ((kOp == kLayerUp && !p.sorted ? p.tokens : x.columns) + kColumnStep - 1) / kColumnStep * kColumnStep;
+    };
+    auto columns_of = [&](const Tile& x, int of, int& from) {
+        if (!kPair) {
+            from = 0;
+            return x.columns;
+        }
+        const int half = product_columns(x) / 2;
+        from = of * half;
+        return max(0, min(half, x.columns - from));
     };
     // kLayer*: a pair's expert, -1 for none
     auto expert_of = [&](int pair) {
@@ -306,18 +329,18 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 const int bytes = whole ? (paired ? 2 : 1) * h1 * kRowBytes : parts_of(h1, piece) * kPieceRows * kRowBytes;
                 int k = block0 * kTileInner;
                 for (int left = blocks; left > 0; left -= per_stage) {
-                    const uint32_t bar = full0 + 8 * stage;
+                    const uint32_t bar = kPair ? of_first_block(full0 + 8 * stage) : full0 + 8 * stage;
                     uint32_t at = ring0 + stage * stage_bytes;
                     if (!barrier_wait(empty0 + 8 * stage, phase, &s.gave_up)) goto weights_done;
                     int n = min(per_stage, left);
-                    barrier_expect(bar, n * bytes);
+                    if (side == 0) barrier_expect(full0 + 8 * stage, n * bytes * kBlocks);
                     for (; n > 0; --n, k += kTileInner, at += block_bytes) {
                         if (whole) {
-                            copy_tile_4d(at, &p.weights, k, 0, f, x.group, bar);
+                            copy_tile_4d<kPair>(at, &p.weights, k, 0, f, x.group, bar);
                         } else {
                             for (int h0 = 0; h0 < h1; h0 += piece) {
                                 const int h = max(0, min(h0, h1 - piece));  // the last one overlaps: the same bytes to the same place
-                                copy_tile_4d(at + h * (paired ? 2 : 1) * kRowBytes, &p.weights_piece, k, 0, f + h, x.group, bar);
+                                copy_tile_4d<kPair>(at + h * (paired ? 2 : 1) * kRowBytes, &p.weights_piece, k, 0, f + h, x.group, bar);
                             }
                         }
                     }
@@ -327,14 +350,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         weights_done:;
         }
     } else if (warp == 1) {
-        if (elect_one()) {
+        if (side == 0 && elect_one()) {
             int stage = 0, n = 0;
             uint32_t phase = 0;
             const uint64_t ring_descriptor = operand_descriptor(ring0);
             for (int t = tile0; t < tiles; t += tile_step, ++n) {
                 const Tile x = tile_of(t);
                 const int buffer = n & 1;
-                const uint32_t descriptor = instruction_descriptor(Element<T>::kFormat, round16(spread ? p.tokens : x.columns));
+                const uint32_t descriptor = instruction_descriptor(Element<T>::kFormat, kTileRows * kBlocks, product_columns(x));
                 const uint32_t sums = tmem + buffer * kMaxColumns;
                 if (!barrier_wait(sums_empty0 + 8 * buffer, ((n >> 1) & 1) ^ 1, &s.gave_up)) goto products_done;
                 tcgen05_after_sync();
@@ -345,16 +368,16 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     for (int b = min(per_stage, left); b > 0; --b, w += block_bytes >> 4) {
                         const uint64_t r = w + (weight_bytes >> 4);
                         // 16 of the inner length are 32 bytes of a row
-                        tcgen05_mma(sums, w, r, descriptor, add);
-                        tcgen05_mma(sums, w + 2, r + 2, descriptor, true);
-                        tcgen05_mma(sums, w + 4, r + 4, descriptor, true);
-                        tcgen05_mma(sums, w + 6, r + 6, descriptor, true);
+                        tcgen05_mma<kPair>(sums, w, r, descriptor, add);
+                        tcgen05_mma<kPair>(sums, w + 2, r + 2, descriptor, true);
+                        tcgen05_mma<kPair>(sums, w + 4, r + 4, descriptor, true);
+                        tcgen05_mma<kPair>(sums, w + 6, r + 6, descriptor, true);
                         add = true;
                     }
-                    tcgen05_commit(empty0 + 8 * stage);
+                    tcgen05_commit<kPair>(empty0 + 8 * stage);
                     if (++stage == stages) stage = 0, phase ^= 1;
                 }
-                tcgen05_commit(sums_full0 + 8 * buffer);
+                tcgen05_commit<kPair>(sums_full0 + 8 * buffer);
             }
         products_done:;
         }
@@ -366,41 +389,45 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             for (int t = tile0; t < tiles; t += tile_step, ++n) {
                 const Tile x = tile_of(t);
                 // the tile's copies of a block of 64: one box, or the boxes of a run, or of the runs of the slabs
-                int bytes = wide * kRowBytes, wide_boxes = 0, some_boxes = 0, boxes = 0, run = 0;
+                int bytes = wide * kRowBytes * kBlocks, wide_boxes = 0, some_boxes = 0, boxes = 0, run = 0, from = 0;  // bytes: of both blocks
+                if (kOp == kDense) columns_of(x, side, from);
                 if (runs) {
-                    run = (x.columns + 7) & ~7;
-                    const int size = run >= 64 ? 64 : run >= 32 ? 32 : 8;
-                    bytes = (run + size - 1) / size * size * kRowBytes;
+                    bytes = 0;
+                    for (int of = 0; of < kBlocks; ++of) {
+                        const int n8 = (columns_of(x, of, from) + 7) & ~7, size = n8 >= 64 ? 64 : n8 >= 32 ? 32 : 8;
+                        bytes += (n8 + size - 1) / size * size * kRowBytes;
+                    }
+                    run = (columns_of(x, side, from) + 7) & ~7;
                 } else if (kOp == kSlabUp) {
                     if (!barrier_wait(list_full0 + 8 * (n & 1), (n >> 1) & 1, &s.gave_up)) goto rows_done;
                     wide_boxes = s.boxes[n & 1][0], some_boxes = s.boxes[n & 1][1], boxes = s.boxes[n & 1][2];
-                    bytes = (64 * wide_boxes + 32 * (some_boxes - wide_boxes) + 8 * (boxes - some_boxes)) * kRowBytes;
+                    bytes = s.box_rows[n & 1] * kRowBytes;
                 }
                 int k = block0 * kTileInner;
                 for (int left = blocks; left > 0; left -= per_stage) {
-                    const uint32_t bar = full0 + 8 * stage;
+                    const uint32_t bar = kPair ? of_first_block(full0 + 8 * stage) : full0 + 8 * stage;
                     uint32_t at = ring0 + stage * stage_bytes + weight_bytes;
                     if (!barrier_wait(empty0 + 8 * stage, phase, &s.gave_up)) goto rows_done;
                     int have = min(per_stage, left);
-                    barrier_expect(bar, have * bytes);
+                    if (side == 0) barrier_expect(full0 + 8 * stage, have * bytes);
                     for (; have > 0; --have, k += kTileInner, at += block_bytes) {
                         if (kOp == kDense || spread) {
-                            copy_tile_2d(at, &p.rows, k, kOp == kDense ? x.first : 0, bar);
+                            copy_tile_2d<kPair>(at, &p.rows, k, kOp == kDense ? x.first + from : 0, bar);
                         } else if (runs) {
-                            const int row = s.row[x.group] + x.first;
+                            const int row = s.row[x.group] + x.first + from;
                             if (run >= 64) {
-                                for (int c = 0; c < run; c += 64) copy_tile_2d(at + min(c, run - 64) * kRowBytes, &p.rows, k, row + min(c, run - 64), bar);
+                                for (int c = 0; c < run; c += 64) copy_tile_2d<kPair>(at + min(c, run - 64) * kRowBytes, &p.rows, k, row + min(c, run - 64), bar);
                             } else if (run >= 32) {
-                                for (int c = 0; c < run; c += 32) copy_tile_2d(at + min(c, run - 32) * kRowBytes, &p.rows_some, k, row + min(c, run - 32), bar);
+                                for (int c = 0; c < run; c += 32) copy_tile_2d<kPair>(at + min(c, run - 32) * kRowBytes, &p.rows_some, k, row + min(c, run - 32), bar);
                             } else {
-                                for (int c = 0; c < run; c += 8) copy_tile_2d(at + c * kRowBytes, &p.rows_few, k, row + c, bar);
+                                for (int c = 0; c < run; c += 8) copy_tile_2d<kPair>(at + c * kRowBytes, &p.rows_few, k, row + c, bar);
                             }
                         } else {
                             const int2* const list = s.box[n & 1];
                             int j = 0;
-                            for (; j < wide_boxes; ++j) copy_tile_2d(at + list[j].y * kRowBytes, &p.rows, k, list[j].x, bar);
-                            for (; j < some_boxes; ++j) copy_tile_2d(at + list[j].y * kRowBytes, &p.rows_some, k, list[j].x, bar);
-                            for (; j < boxes; ++j) copy_tile_2d(at + list[j].y * kRowBytes, &p.rows_few, k, list[j].x, bar);
+                            for (; j < wide_boxes; ++j) copy_tile_2d<kPair>(at + list[j].y * kRowBytes, &p.rows, k, list[j].x, bar);
+                            for (; j < some_boxes; ++j) copy_tile_2d<kPair>(at + list[j].y * kRowBytes, &p.rows_some, k, list[j].x, bar);
+                            for (; j < boxes; ++j) copy_tile_2d<kPair>(at + list[j].y * kRowBytes, &p.rows_few, k, list[j].x, bar);
                         }
                     }
                     if (++stage == stages) stage = 0, phase ^= 1;
@@ -453,23 +480,30 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     __syncwarp();
                     // Every eight columns begin with a row; lane i looks at columns 8 i to 8 i + 7, where its run begins and ends, and
                     // whether a box begins there.
-                    const int eights = x.columns >> 3, row = lane < eights ? s.list[buffer][8 * lane] : -1;
-                    const int before = __shfl_up_sync(0xffffffffu, row, 1);
-                    const unsigned breaks = __ballot_sync(0xffffffffu, lane == 0 || lane >= eights || row != before + 8);
-                    const int run0 = 31 - __clz(breaks & (0xffffffffu >> (31 - lane)));
-                    const unsigned later = lane == 31 ? 0 : breaks >> (lane + 1);
-                    const int run1 = later ? lane + __ffs(later) : 32;
-                    const int run = run1 - run0, place = lane - run0, size = run >= 8 ? 8 : run >= 4 ? 4 : 1;
-                    const bool begins = lane < eights && ((place % size == 0 && place + size <= run) || place == run - size);
-                    int boxes = 0;
+                    int box_rows = 0;
+                    for (int of = 0; of < kBlocks; ++of) {
+                        int from;
+                        const int eights = columns_of(x, of, from) >> 3, row = lane < eights ? s.list[buffer][from + 8 * lane] : -1;
+                        const int before = __shfl_up_sync(0xffffffffu, row, 1);
+                        const unsigned breaks = __ballot_sync(0xffffffffu, lane == 0 || lane >= eights || row != before + 8);
+                        const int run0 = 31 - __clz(breaks & (0xffffffffu >> (31 - lane)));
+                        const unsigned later = lane == 31 ? 0 : breaks >> (lane + 1);
+                        const int run1 = later ? lane + __ffs(later) : 32;
+                        const int run = run1 - run0, place = lane - run0, size = run >= 8 ? 8 : run >= 4 ? 4 : 1;
+                        const bool begins = lane < eights && ((place % size == 0 && place + size <= run) || place == run - size);
+                        int boxes = 0;
 #pragma unroll
-                    for (int kind = 0; kind < 3; ++kind) {
-                        const bool mine = begins && size == (kind == 0 ? 8 : kind == 1 ? 4 : 1);
-                        const unsigned all = __ballot_sync(0xffffffffu, mine);
-                        if (mine) s.box[buffer][boxes + __popc(all & ((1u << lane) - 1))] = make_int2(row, 8 * lane);
-                        boxes += __popc(all);
-                        if (lane == 0) s.boxes[buffer][kind] = boxes;
+                        for (int kind = 0; kind < 3; ++kind) {
+                            const int rows = kind == 0 ? 8 : kind == 1 ? 4 : 1;
+                            const bool mine = begins && size == rows;
+                            const unsigned all = __ballot_sync(0xffffffffu, mine);
+                            if (of == side && mine) s.box[buffer][boxes + __popc(all & ((1u << lane) - 1))] = make_int2(row, 8 * lane);
+                            boxes += __popc(all);
+                            box_rows += 8 * rows * __popc(all);
+                            if (of == side && lane == 0) s.boxes[buffer][kind] = boxes;
+                        }
                     }
+                    if (lane == 0) s.box_rows[buffer] = box_rows;
                 }
                 __syncwarp();
                 if (lane == 0) barrier_arrive(list_full0 + 8 * buffer);
@@ -482,7 +516,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             cudaTriggerProgrammaticLaunchCompletion();
         }
         int n = 0;
-        bool met = kOp != kDense || split == 1;
+        bool met = kOp != kDense || kPair || split == 1;
         for (int t = tile0; t < tiles; t += tile_step, ++n) {
             const Tile x = tile_of(t);
             const int buffer = n & 1;
@@ -557,7 +591,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     }
                 }
             };
-            if (kOp == kDense && split > 1) {
+            if (kOp == kDense && !kPair && split > 1) {
                 // The cluster's blocks leave their sums in the ring, which nothing uses any more, and each finishes its share of the
                 // columns, two at a time.
                 float* const left = reinterpret_cast<float*>(ring);
@@ -588,7 +622,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             }
             tcgen05_before_sync();
             __syncwarp();
-            if (lane == 0) barrier_arrive(sums_empty0 + 8 * buffer);
+            if (lane == 0) kPair ? barrier_arrive_there(of_first_block(sums_empty0 + 8 * buffer)) : barrier_arrive(sums_empty0 + 8 * buffer);
             if (kGrouped) {
                 named_sync(1, kFinishers);
                 if (at == 0) barrier_arrive(list_empty0 + 8 * buffer);
@@ -598,12 +632,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     }
     __syncwarp();
     // What the epilogue's threads meet at, the others meet here: nobody leaves while its sums are read.
-    if (kOp == kDense && split > 1) {
+    if (kOp == kDense && !kPair && split > 1) {
         if (warp < 4) cluster_sync();
         cluster_sync();
     }
     tcgen05_before_sync();
     __syncthreads();
+    if (kPair) cluster_sync();  // the other block's products and arrivals have come here
     tcgen05_after_sync();
     if (s.gave_up) {
         // copies and products in flight end in less than this
@@ -612,7 +647,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         if (tid == 0) atomicExch(&g_product_error, A2A_ERR_TIMEOUT);
         __syncthreads();
     }
-    if (warp == 1) tmem_free(tmem, kTmemColumns);
+    if (warp == 1) tmem_free<kPair>(tmem, kTmemColumns);
 }
 
 // The rows of a layer's pairs by expert, and within an expert in the order of the pairs: a warp a pair, which counts the pairs before its own
