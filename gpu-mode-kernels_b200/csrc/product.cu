@@ -184,6 +184,7 @@ int linear_of(const a2a_linear_args& a, int sms, cudaStream_t st) {
     p.inner = a.inputs, p.features = a.outputs, p.paired = paired, p.groups = 1, p.tokens = a.tokens;
     p.activation = a.activation, p.out_fp32 = a.out_dtype == A2A_DTYPE_FP32, p.bias_fp32 = a.bias_dtype == A2A_DTYPE_FP32;
     p.bias = a.bias, p.residual = a.residual, p.residual_stride = a.residual_stride, p.y = a.y, p.y_stride = a.y_stride;
+    p.wide_stores = a.y_stride % 8 == 0 && aligned(a.y) && (a.residual == nullptr || (a.residual_stride % 8 == 0 && aligned(a.residual)));
     const DensePlan plan = dense_plan<T>(a, paired, sms);
     p.columns = plan.columns, p.full = plan.height, p.split = plan.split;
     int rc = weights_map(&p.weights, a.dtype, a.weight, 1, a.outputs, paired, a.inputs, a.weight_stride, plan.height);
@@ -237,6 +238,7 @@ int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
     TilesParams p{};
     p.groups = a.experts, p.tokens = a.tokens, p.topk = a.topk, p.indices = a.topk_idx, p.weights_of = a.topk_weights;
     p.hidden = space, p.parts = reinterpret_cast<float*>(space + at.parts);
+    p.wide_stores = 1;
     p.columns = kMaxColumns;
     int rc = expert_maps(p, a.dtype, a.gate_up, a.experts, a.inner, true, a.hidden_dim);
     p.sorted = a.tokens > kSpreadTokens;
@@ -264,13 +266,13 @@ template <typename T>
 int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {
     const long long rows = (long long)a.local_experts * a.world * a.capacity;
     TilesParams p{};
-    p.groups = a.local_experts, p.counts = a.counts, p.world = a.world, p.capacity = a.capacity, p.hidden = a.workspace;
+    p.groups = a.local_experts, p.counts = a.counts, p.world = a.world, p.capacity = a.capacity, p.hidden = a.workspace, p.wide_stores = 1;
     p.columns = kMaxColumns;
     int rc = expert_maps(p, a.dtype, a.gate_up, a.local_experts, a.inner, true, a.hidden_dim);
     if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.rows, rows);
     if (rc == A2A_OK) rc = launch_tiles<kSlabUp, T, true>(p, 2 * std::max(1, most_clusters<kSlabUp, T, true>(2)), 2, st);
     if (rc != A2A_OK) return rc;
-    p.y = a.out;
+    p.y = a.out, p.wide_stores = aligned(a.out);
     rc = expert_maps(p, a.dtype, a.down, a.local_experts, a.hidden_dim, false, a.inner);
     if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.workspace, inner_rows(a.local_experts, a.world, a.capacity));
     return rc == A2A_OK ? launch_tiles<kSlabDown, T, true>(p, 2 * std::max(1, most_clusters<kSlabDown, T, true>(2)), 2, st) : rc;

@@ -51,6 +51,51 @@ __device__ __forceinline__ void store_any(void* p, size_t i, float v, bool fp32)
         static_cast<T*>(p)[i] = Element<T>::from_float(v);
 }
 
+// Eight values from a place on 16 bytes, added to `v`; and to one.
+template <typename T>
+__device__ __forceinline__ void add_eight(float (&v)[8], const void* p, size_t i, bool fp32) {
+    if (fp32) {
+        const float4* const at = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        const float4 a = at[0], b = at[1];
+        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+    } else {
+        const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const T*>(p) + i);
+        const T* const e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += Element<T>::to_float(e[j]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void put_eight(void* p, size_t i, const float (&v)[8], bool fp32) {
+    if (fp32) {
+        float4* const at = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+        at[0] = make_float4(v[0], v[1], v[2], v[3]);
+        at[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        alignas(16) T e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = Element<T>::from_float(v[j]);
+        *reinterpret_cast<uint4*>(static_cast<T*>(p) + i) = *reinterpret_cast<const uint4*>(e);
+    }
+}
+// Lanes that differ in the three bits from kStep on, and their eight values, change places: value i of the lane whose bits are j was value j of the
+// one whose bits are i.
+template <int kStep>
+__device__ __forceinline__ void exchange_eight(float (&v)[8], int lane) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        const bool high = lane & kStep << k;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i >> k & 1) continue;
+            const int j = i | 1 << k;
+            const float got = __shfl_xor_sync(0xffffffffu, high ? v[i] : v[j], kStep << k);
+            v[i] = high ? got : v[i];
+            v[j] = high ? v[j] : got;
+        }
+    }
+}
+
 // ---- the epilogue's arithmetic: fp32, on the fp32 sums of a product -------------------------------
 // (The quick division gives 0 where the divisor is above 2^126: below -87, where silu is less than 1e-35.)
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + expf(-v)); }
