@@ -247,7 +247,7 @@ int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
         // where the second product will have its rows of pairs, which are wider
         rc = run_maps(p, a.dtype, p.parts, (long long)a.tokens * a.topk);
         SortParams sort{a.x, a.topk_idx, p.parts, a.tokens, a.topk, a.experts, a.hidden_dim * 2};
-        if (rc == A2A_OK) rc = launch(reinterpret_cast<const void*>(&layer_rows_kernel), parts_of(a.tokens * a.topk, kSortThreads / 32), kSortThreads, 0, 1, &sort, st);
+        if (rc == A2A_OK) rc = launch(reinterpret_cast<const void*>(&layer_rows_kernel), a.tokens * a.topk, kSortThreads, 0, 1, &sort, st);
     }
     if (rc == A2A_OK) rc = launch_tiles<kLayerUp, T>(p, sms, 1, st);
     if (rc != A2A_OK) return rc;

@@ -19,7 +19,7 @@
 // made a step of 64 take 1230 cycles where the weights' bytes take 700.)
 //
 // The second product of a layer leaves a row a pair, in fp32, and a launch of its own adds a token's rows up: tickets, by which the tile that
-// brings a token's last row adds them, took 3 us a tile (64 tokens of 2048 146 us a layer where this takes 130; 256 of 4096 740 and 680).
+// brings a token's last row adds them, took 3 us a tile (64 tokens of 2048, top-6 of 64: 146 us a layer where this takes 129).
 //
 // Roles of the twelve warps: 0 weights, 1 products, 2 rows, 3 the lists of rows, 4 to 11 the epilogue, two for each 32 lanes of the tensor
 // memory: every other 16 columns each.
@@ -462,10 +462,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                             if (e[j] == x.group && at >= 0 && at < x.columns) {
                                 const int pair = i0 + 32 * j + lane;
                                 s.list[buffer][at] = pair;
-                                if (kOp == kLayerDown) s.scale[buffer][at] = p.weights_of[pair];
                             }
                             seen += __popc(mine);
                         }
+                    }
+                    if (kOp == kLayerDown) {
+                        __syncwarp();
+                        for (int c = lane; c < x.columns; c += 32) s.scale[buffer][c] = p.weights_of[s.list[buffer][c]];
                     }
                 } else {
                     for (int c = lane; c < x.columns; c += 32) {
@@ -709,9 +712,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     if (warp == 1) tmem_free<kPair>(tmem, kTmemColumns);
 }
 
-// The rows of a layer's pairs by expert, and within an expert in the order of the pairs: a warp a pair, which counts the pairs before its own
-// and copies the token's row. 256 tokens of 4096, top-8: 34 MB moved for 1.1 GB of weights that follow.
-constexpr int kSortThreads = 256;
+// The rows of a layer's pairs by expert, and within an expert in the order of the pairs: a block a pair, which counts the pairs before its own
+// and copies the token's row. (A warp a pair: 18 us for 2048 of 4096, instead of 9.)
+constexpr int kSortThreads = 128;
 struct SortParams {
     const void* x;
     const int* indices;
@@ -719,21 +722,27 @@ struct SortParams {
     int tokens, topk, experts, row_bytes;
 };
 __global__ void __launch_bounds__(kSortThreads) layer_rows_kernel(const SortParams p) {
+    __shared__ int counted[kSortThreads / 32];
     cudaGridDependencySynchronize();
     cudaTriggerProgrammaticLaunchCompletion();
-    const int pairs = p.tokens * p.topk, pair = blockIdx.x * (kSortThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (pair >= pairs) return;
+    const int pairs = p.tokens * p.topk, pair = blockIdx.x, tid = threadIdx.x;
     const int own = p.indices[pair];
     if (own < 0 || own >= p.experts) return;
     int before = 0;
-    for (int i = lane; i < pairs; i += 32) {
+#pragma unroll 8
+    for (int i = tid; i < pairs; i += kSortThreads) {
         const int e = p.indices[i];
         before += e >= 0 && (e < own || (e == own && i < pair));
     }
     before = __reduce_add_sync(0xffffffffu, before);
+    if ((tid & 31) == 0) counted[tid >> 5] = before;
+    __syncthreads();
+    before = 0;
+    for (int w = 0; w < kSortThreads / 32; ++w) before += counted[w];
     const uint4* const from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.x) + (size_t)(pair / p.topk) * p.row_bytes);
     uint4* const to = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.rows) + (size_t)before * p.row_bytes);
-    for (int i = lane; i < p.row_bytes / 16; i += 32) to[i] = from[i];
+#pragma unroll 4
+    for (int i = tid; i < p.row_bytes / 16; i += kSortThreads) to[i] = from[i];
 }
 
 // y[t] = residual[t] + the rows of the token's pairs, in the order of its choices; a thread four features.
