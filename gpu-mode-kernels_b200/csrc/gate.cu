@@ -67,23 +67,26 @@ __global__ void __launch_bounds__(kThreads) gate_kernel(const GateParams p) {
     const int token = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (token >= p.tokens) return;
     const T* const row = static_cast<const T*>(p.logits) + token * p.stride;
+    // (unrolled by number: left to itself the compiler keeps 64-bit scores in local memory, 8.0 us for 2048 tokens of 256 instead of 7.2)
     V score[kOwn];
     Key key[kOwn];
-#pragma unroll
+    float bias[sizeof(V) == 8 ? kOwn : 1];
+#pragma unroll kOwn
     for (int j = 0; j < kOwn; ++j) {
         const int e = 32 * j + lane;
         score[j] = e < p.experts ? (V)as_float(row[e]) : (V)-INFINITY;
         key[j] = 0;
         if (sizeof(V) == 4 && e < p.experts) key[j] = key_of(score[j]);
+        if constexpr (sizeof(V) == 8) bias[j] = e < p.experts ? p.bias[e] : 0.0f;
     }
     V total = 1;
     if (p.sigmoid) {
-#pragma unroll
+#pragma unroll kOwn
         for (int j = 0; j < kOwn; ++j) score[j] = (V)1 / ((V)1 + exponential(-score[j]));
     } else {
         V most = score[0];
         bool nan = score[0] != score[0];
-#pragma unroll
+#pragma unroll kOwn
         for (int j = 1; j < kOwn; ++j) {
             most = score[j] > most ? score[j] : most;
             nan = nan || score[j] != score[j];
@@ -94,7 +97,7 @@ __global__ void __launch_bounds__(kThreads) gate_kernel(const GateParams p) {
         }
         if (__any_sync(0xffffffffu, nan)) most = (V)NAN;
         V sum = 0;
-#pragma unroll
+#pragma unroll kOwn
         for (int j = 0; j < kOwn; ++j) {
             // a row of nothing but -inf has no scores: zeros
             score[j] = most == (V)-INFINITY ? (V)0 : exponential(score[j] - most);
@@ -103,17 +106,18 @@ __global__ void __launch_bounds__(kThreads) gate_kernel(const GateParams p) {
         total = warp_sum(sum);
     }
     const V share = p.sigmoid || total == 0 ? (V)1 : (V)1 / total;
-#pragma unroll
+#pragma unroll kOwn
     for (int j = 0; j < kOwn; ++j) {
         score[j] *= share;
         const int e = 32 * j + lane;
-        if (sizeof(V) == 8 && e < p.experts) key[j] = key_of(score[j] + (V)p.bias[e]);
+        if constexpr (sizeof(V) == 8)
+            if (e < p.experts) key[j] = key_of(score[j] + (V)bias[j]);
     }
 
     // this lane's best, the lowest index among equals
     auto best_of = [&](Key& best, int& at, V& value) {
         best = key[0], at = 0, value = score[0];
-#pragma unroll
+#pragma unroll kOwn
         for (int j = 1; j < kOwn; ++j)
             if (key[j] > best) best = key[j], at = j, value = score[j];
     };
@@ -129,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) gate_kernel(const GateParams p) {
         sum += got;
         if (lane == k) chosen = (int)e, mine = got;
         if (lane == (e & 31)) {
-#pragma unroll
+#pragma unroll kOwn
             for (int j = 0; j < kOwn; ++j)
                 if (j == (int)(e >> 5)) key[j] = 0;
             best_of(best, at, value);
