@@ -29,7 +29,7 @@ GROUP_PHASE = {"pipe_send": 0, "pipe_expert": 1, "pipe_combine": 2, "send": 3, "
 ACTIVATION = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "swiglu": 4}
 SCORE = {"softmax": 0, "sigmoid": 1}
 MAX_WORLD, MAX_EXPERTS, MAX_TOPK = 8, 1024, 32
-MAX_PRODUCT, MAX_LAYER_TOKENS = 65536, 256
+MAX_PRODUCT, MAX_OUTPUTS, MAX_ROWS, MAX_LAYER_TOKENS = 65536, 1 << 24, 1 << 30, 256
 
 
 class Config(C.Structure):

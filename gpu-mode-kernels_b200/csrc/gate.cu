@@ -162,7 +162,7 @@ extern "C" int a2a_gate(const a2a_gate_args* args, void* stream) {
     if (args == nullptr) return A2A_ERR_CONFIG;
     const a2a_gate_args& a = *args;
     if (a.dtype != A2A_DTYPE_BF16 && a.dtype != A2A_DTYPE_FP16 && a.dtype != A2A_DTYPE_FP32) return A2A_ERR_CONFIG;
-    if (a.tokens < 0 || a.experts < 1 || a.experts > A2A_MAX_EXPERTS || a.topk < 1 || a.topk > A2A_MAX_TOPK || a.topk > a.experts) return A2A_ERR_CONFIG;
+    if (a.tokens < 0 || a.tokens > A2A_MAX_ROWS || a.experts < 1 || a.experts > A2A_MAX_EXPERTS || a.topk < 1 || a.topk > A2A_MAX_TOPK || a.topk > a.experts) return A2A_ERR_CONFIG;
     if (a.score != A2A_SCORE_SOFTMAX && a.score != A2A_SCORE_SIGMOID) return A2A_ERR_CONFIG;
     if (a.tokens == 0) return A2A_OK;
     if (a.logits == nullptr || a.indices == nullptr || a.weights == nullptr || a.stride < 0) return A2A_ERR_CONFIG;

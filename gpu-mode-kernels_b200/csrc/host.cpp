@@ -252,7 +252,7 @@ PyObject* gate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     int device;
     const at::Tensor* logits = here(args[0], &device);
-    if (logits == nullptr || logits->dim() != 2 || logits->size(0) > INT32_MAX || !PyLong_CheckExact(args[1]) || !PyUnicode_CheckExact(args[2]) || !PyBool_Check(args[4]) ||
+    if (logits == nullptr || logits->dim() != 2 || logits->size(0) > A2A_MAX_ROWS || !PyLong_CheckExact(args[1]) || !PyUnicode_CheckExact(args[2]) || !PyBool_Check(args[4]) ||
         !PyFloat_CheckExact(args[5]))
         Py_RETURN_NONE;
     if (!sixteen(logits->scalar_type()) && logits->scalar_type() != at::kFloat) Py_RETURN_NONE;
@@ -294,11 +294,11 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     int device;
     const at::Tensor* x = here(args[0], &device);
-    if (x == nullptr || x->dim() != 2 || !sixteen(x->scalar_type()) || x->size(0) > INT32_MAX || !PyUnicode_CheckExact(args[3])) Py_RETURN_NONE;
+    if (x == nullptr || x->dim() != 2 || !sixteen(x->scalar_type()) || x->size(0) > A2A_MAX_ROWS || !PyUnicode_CheckExact(args[3])) Py_RETURN_NONE;
     const at::ScalarType dtype = x->scalar_type();
     const int64_t tokens = x->size(0), inputs = x->size(1);
     const at::Tensor* weight = matrix(args[1], dtype, device, -1, inputs);
-    if (weight == nullptr || inputs > A2A_MAX_PRODUCT || weight->size(0) > 2 * A2A_MAX_PRODUCT) Py_RETURN_NONE;
+    if (weight == nullptr || inputs > A2A_MAX_PRODUCT || weight->size(0) > 2 * A2A_MAX_OUTPUTS) Py_RETURN_NONE;
     const char* const names[] = {"none", "relu", "gelu", "silu", "swiglu"};
     a2a_linear_args a{};
     for (a.activation = 0; a.activation <= A2A_ACT_SWIGLU; ++a.activation)

@@ -302,7 +302,7 @@ extern "C" int a2a_linear(const a2a_linear_args* args, void* stream) {
     if (!dtype16(a.dtype) || (a.out_dtype != a.dtype && a.out_dtype != A2A_DTYPE_FP32)) return A2A_ERR_CONFIG;
     if (a.bias != nullptr && a.bias_dtype != a.dtype && a.bias_dtype != A2A_DTYPE_FP32) return A2A_ERR_CONFIG;
     if (a.activation < A2A_ACT_NONE || a.activation > A2A_ACT_SWIGLU) return A2A_ERR_CONFIG;
-    if (a.tokens < 0 || a.outputs < 1 || a.outputs > A2A_MAX_PRODUCT || a.inputs < 8 || a.inputs % 8 != 0 || a.inputs > A2A_MAX_PRODUCT)
+    if (a.tokens < 0 || a.tokens > A2A_MAX_ROWS || a.outputs < 1 || a.outputs > A2A_MAX_OUTPUTS || a.inputs < 8 || a.inputs % 8 != 0 || a.inputs > A2A_MAX_PRODUCT)
         return A2A_ERR_CONFIG;
     if (a.tokens == 0) return A2A_OK;
     if (a.x == nullptr || a.weight == nullptr || a.y == nullptr || !aligned(a.x) || !aligned(a.weight)) return A2A_ERR_CONFIG;

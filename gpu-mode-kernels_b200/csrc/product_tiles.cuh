@@ -86,6 +86,37 @@ struct TilesParams {
     int world, capacity;
 };
 
+// a / b for a >= 0, b > 0. A block works out a dozen of them, one after the other, before its first copy is on its way: an integer division is
+// 100 cycles and more, this half of that. (The quotient of a + 1/2 is at least 1/(2 b) away from a whole number, and __fdividef
+// is off by 2^-22 of it.)
+__host__ __device__ __forceinline__ int quotient(int a, int b) {
+#ifdef __CUDA_ARCH__
+    if (a < 1 << 20) return (int)__fdividef((float)a + 0.5f, (float)b);
+#endif
+    return a / b;
+}
+__host__ __device__ __forceinline__ int parts_of(int n, int size) { return quotient(n + size - 1, size); }
+
+// How `tiles` tiles of `height` features go over `blocks` blocks: whole rounds, and those of the last round in `cut` parts of `part` features.
+struct Rounds {
+    int whole, cut, part;
+};
+// least: a power of two
+__host__ __device__ __forceinline__ Rounds rounds_of(int tiles, int blocks, int height, int least) {
+    constexpr int step = 8;
+    Rounds r;
+    r.whole = quotient(tiles, blocks);
+    const int rest = tiles - r.whole * blocks;
+    r.cut = rest > 0 ? max(1, min(quotient(blocks, rest), height / least)) : 1;
+    r.part = height;
+    if (r.cut > 1) {
+        r.part = (parts_of(height, r.cut) + step - 1) & -step;
+        r.cut = parts_of(height, r.part);
+    }
+    return r;
+}
+
+
 struct TilesShared {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t sums_full[2], sums_empty[2];
@@ -93,7 +124,8 @@ struct TilesShared {
     uint32_t tmem;
     int gave_up;
     int largest;  // columns of the largest group
-    int height;
+    int height, tiles;
+    Rounds rounds;
     int begin[kMaxGroups + 1];  // tiles of one feature tile before a group's
     int count[kMaxGroups];      // columns of a group
     int row[kMaxGroups];        // columns before a group's
@@ -114,24 +146,6 @@ struct Tile {
     int group, f, height, first, columns;  // matrix, first feature, features, first column, columns
 };
 
-__host__ __device__ __forceinline__ int parts_of(int n, int size) { return (n + size - 1) / size; }
-
-// How `tiles` tiles of `height` features go over `blocks` blocks: whole rounds, and those of the last round in `cut` parts of `part` features.
-struct Rounds {
-    int whole, cut, part;
-};
-__host__ __device__ __forceinline__ Rounds rounds_of(int tiles, int blocks, int height, int least, int step) {
-    Rounds r;
-    r.whole = tiles / blocks;
-    const int rest = tiles - r.whole * blocks;
-    r.cut = rest > 0 ? max(1, min(blocks / rest, height / least)) : 1;
-    r.part = height;
-    if (r.cut > 1) {
-        r.part = (parts_of(height, r.cut) + step - 1) & -step;  // step: a power of two
-        r.cut = parts_of(height, r.part);
-    }
-    return r;
-}
 
 __host__ __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
 // What a block of 64 of a tile takes, in ns: the SM's share of the memory's rate for the weights (6.5 TB/s over 148), what the L2 gives an SM
@@ -222,10 +236,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             // the height whose tiles take the fullest SM least: a whole box, or a lane a multiple of 8 from a piece on
             const int piece = kPieceRows / (kUp ? 2 : 1), h = lane == 31 ? p.full : 8 * (lane + 1);
             unsigned cost = 0xffffffffu;
+            int tiles = 0;
+            Rounds r{};
             if ((h >= piece && h < p.full) || lane == 31) {
                 const int wide = kOp == kLayerUp && !p.sorted ? round16(p.tokens) : columns;
-                const int tiles = run * parts_of(p.features, kBlocks * h);
-                const Rounds r = rounds_of(tiles, units, h, piece, 8);
+                tiles = run * parts_of(p.features, kBlocks * h);
+                r = rounds_of(tiles, units, h, piece);
                 // (pieces have to be issued: 30 ns)
                 float ns = r.whole * (block_ns(h * (kUp ? 2 : 1), wide, wide / kBlocks, 1.0f / 44) + (h < p.full ? 30.0f : 0.0f));
                 if (r.whole * units < tiles) ns += block_ns(r.part * (kUp ? 2 : 1), wide, wide / kBlocks, 1.0f / 44) + (r.part < p.full ? 30.0f : 0.0f);
@@ -233,7 +249,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             }
             const unsigned least = __reduce_min_sync(0xffffffffu, cost);
             const int best = 31 - __clz(__ballot_sync(0xffffffffu, cost == least));  // the highest of the best
-            if (lane == 0) s.begin[p.groups] = run, s.height = best == 31 ? p.full : 8 * (best + 1);
+            if (lane == best) s.begin[p.groups] = run, s.height = h, s.tiles = tiles, s.rounds = r;
         }
     }
     tcgen05_before_sync();
@@ -245,19 +261,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     const uint32_t full0 = shared_addr(s.full), empty0 = shared_addr(s.empty), sums_full0 = shared_addr(s.sums_full), sums_empty0 = shared_addr(s.sums_empty),
                    list_full0 = shared_addr(s.list_full), list_empty0 = shared_addr(s.list_empty), ring0 = shared_addr(ring);
     const int feature_tiles = parts_of(p.features, kBlocks * height);
-    const int across_all = kGrouped ? s.begin[p.groups] : parts_of(p.tokens, columns);
+    const int full_tiles = kGrouped ? s.tiles : parts_of(p.tokens, columns) * feature_tiles;
     // over experts: the tiles that come in whole rounds, and the others in parts
     const int piece = kPieceRows / (paired ? 2 : 1);
-    const Rounds rounds = kGrouped ? rounds_of(across_all * feature_tiles, units, height, piece, 8) : Rounds{0, 1, height};
+    const Rounds rounds = kGrouped ? s.rounds : Rounds{0, 1, height};
     const int whole_tiles = kGrouped ? rounds.whole * units : 0;
-    const int tiles = whole_tiles + (across_all * feature_tiles - whole_tiles) * rounds.cut;
+    const int tiles = whole_tiles + (full_tiles - whole_tiles) * rounds.cut;
     // the operand's columns in a stage, of this block
     const int wide = kOp == kLayerUp && !p.sorted ? round16(p.tokens) : columns / kBlocks;
     const int highest = whole_tiles > 0 ? height : rounds.part;
     const int weight_bytes = ((paired ? 2 : 1) * max(highest, kGrouped ? piece : 0) * kRowBytes + 1023) & ~1023, block_bytes = weight_bytes + wide * kRowBytes;
     const int blocks_all = parts_of(p.inner, kTileInner);
-    const int per_stage = min(blocks_all, max(1, (kStageBytes + block_bytes / 2) / block_bytes));
-    const int stages = min(kMaxStages, kRingBytes / (block_bytes * per_stage));
+    const int per_stage = min(blocks_all, max(1, quotient(kStageBytes + block_bytes / 2, block_bytes)));
+    const int stages = min(kMaxStages, quotient(kRingBytes, block_bytes * per_stage));
     // this block's part of the inner length, and its tiles
     const int split = kOp == kDense && !kPair ? p.split : 1, part = kOp == kDense && !kPair ? (int)blockIdx.x % split : 0;
     const int block0 = blocks_all * part / split, blocks = blocks_all * (part + 1) / split - block0;
@@ -269,13 +285,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         int count, cut = 0;
         x.height = height;
         if (t >= whole_tiles && rounds.cut > 1) {
-            const int q = (t - whole_tiles) / rounds.cut;
+            const int q = quotient(t - whole_tiles, rounds.cut);
             cut = (t - whole_tiles - q * rounds.cut) * rounds.part;
             t = whole_tiles + q;
             x.height = min(rounds.part, height - cut);
         }
         if (kGrouped) {
-            const int q = t / feature_tiles;
+            const int q = quotient(t, feature_tiles);
             int lo = 0, hi = p.groups - 1;  // the last group that begins at or before q; groups without rows begin with the next
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
@@ -290,7 +306,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             count = p.tokens;
         }
         const int across = parts_of(count, columns);
-        const int m = t / across;
+        const int m = quotient(t, across);
         x.f = kBlocks * (m * height + cut) + side * x.height;  // this block's
 
         x.first = (t - m * across) * columns;

@@ -59,8 +59,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     outputs = rows // 2 if activation == "swiglu" else rows
     if outputs == 0 or (activation == "swiglu" and rows % 2):
         refuse(f"weight has {rows} rows" + (", and swiglu takes an even number: gate rows and up rows" if rows else ""))
-    if inputs < 8 or inputs % 8 or max(inputs, outputs) > _lib.MAX_PRODUCT:
-        refuse(f"inputs must be a multiple of 8, inputs and outputs at most {_lib.MAX_PRODUCT}, got {inputs} and {outputs}")
+    if inputs < 8 or inputs % 8 or inputs > _lib.MAX_PRODUCT or outputs > _lib.MAX_OUTPUTS:
+        refuse(f"inputs must be a multiple of 8 up to {_lib.MAX_PRODUCT}, outputs at most {_lib.MAX_OUTPUTS}, got {inputs} and {outputs}")
     out_dtype = out_dtype or x.dtype
     if out_dtype not in (x.dtype, torch.float32):
         refuse(f"out_dtype must be {x.dtype} or torch.float32, got {out_dtype}")
@@ -82,6 +82,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     tokens = flat.shape[0]
     if tokens == 0:
         return y
+    if tokens > _lib.MAX_ROWS:
+        refuse(f"at most {_lib.MAX_ROWS} rows, got {tokens}")
     add = None
     if residual is not None:
         add = residual if residual.dim() == 2 else residual.reshape(-1, outputs)

@@ -1,7 +1,7 @@
 """The layer around the all-to-all: the gate that chooses a token's experts, and the experts themselves.
 
 ``topk_gate``   indices and weights, as ``custom_kernel`` and ``A2AContext`` take them, from the router's logits.
-``moe_layer``   a whole layer for a few tokens on one GPU: experts' products and their weighted sum in two launches.
+``moe_layer``   a whole layer for a few tokens on one GPU: experts' products and their weighted sum.
 ``expert_mlp``  the experts' products on the rows a dispatch has left: the real expert op between ``A2AContext.dispatch_recv``
                 and ``expert_done`` (``A2AContext.experts`` calls it there).
 
@@ -43,8 +43,8 @@ def topk_gate(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Opt
         with torch.cuda.device(device):
             return topk_gate(logits, k, score=score, bias=bias, renormalize=renormalize, scale=scale)
     tokens, experts = logits.shape
-    if not 1 <= experts <= _lib.MAX_EXPERTS or not 1 <= k <= min(experts, _lib.MAX_TOPK):
-        refuse(f"1 to {_lib.MAX_EXPERTS} experts, and 1 to {_lib.MAX_TOPK} of them chosen, not {k} of {experts}")
+    if tokens > _lib.MAX_ROWS or not 1 <= experts <= _lib.MAX_EXPERTS or not 1 <= k <= min(experts, _lib.MAX_TOPK):
+        refuse(f"1 to {_lib.MAX_EXPERTS} experts, and 1 to {_lib.MAX_TOPK} of them chosen, not {k} of {experts}; at most {_lib.MAX_ROWS} tokens")
     if score not in _lib.SCORE:
         refuse(f"score must be one of {', '.join(_lib.SCORE)}, got {score!r}")
     if bias is not None and (bias.dtype is not torch.float32 or tuple(bias.shape) != (experts,) or not bias.is_contiguous()

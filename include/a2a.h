@@ -355,8 +355,8 @@ size_t a2a_symmetric_bytes(a2a_ctx* ctx);
 enum { A2A_DTYPE_FP32 = 2 };
 enum { A2A_ACT_NONE = 0, A2A_ACT_RELU = 1, A2A_ACT_GELU = 2, A2A_ACT_SILU = 3, A2A_ACT_SWIGLU = 4 };
 enum { A2A_SCORE_SOFTMAX = 0, A2A_SCORE_SIGMOID = 1 };
-/* longest row of a matrix and most rows of one (twice that with SwiGLU); most tokens of a2a_layer */
-enum { A2A_MAX_PRODUCT = 65536, A2A_MAX_LAYER_TOKENS = 256 };
+/* longest row of a matrix, and inner size of an expert; most outputs and most rows of x of a dense product; most tokens of a2a_layer */
+enum { A2A_MAX_PRODUCT = 65536, A2A_MAX_OUTPUTS = 1 << 24, A2A_MAX_ROWS = 1 << 30, A2A_MAX_LAYER_TOKENS = 256 };
 
 /* Gate: indices and weights [tokens, topk] from logits [tokens, experts] (rows `stride` apart), as a2a_route and a2a_forward take
  * them.  score s = softmax or sigmoid of the logits; chosen are the topk largest logits, or, with a bias [experts], the largest s + bias
@@ -386,7 +386,8 @@ typedef struct a2a_linear_args {
 } a2a_linear_args;
 int a2a_linear(const a2a_linear_args* args, void* stream);
 
-/* A whole layer of a few tokens (at most A2A_MAX_LAYER_TOKENS) on one GPU, in two launches: y[t] = residual[t] + sum over k of w[t, k] *
+/* A whole layer of a few tokens (at most A2A_MAX_LAYER_TOKENS) on one GPU, two products and the sum of a token's experts (above 64 tokens
+ * a sort of the rows in front): y[t] = residual[t] + sum over k of w[t, k] *
  * down_e (silu(gate_e x[t]) * up_e x[t]), e = topk_idx[t, k]; gate_up [experts, 2 inner, hidden_dim] (gate rows before up rows),
  * down [experts, hidden_dim, inner], all contiguous.  An index outside 0..experts-1 marks no expert; the same expert twice counts twice.
  * y overlaps no input but residual, which it may be. */

@@ -1,12 +1,14 @@
 """The gate, the products and the all-to-all together, as a model's layer runs them; streams, graphs, other devices, calls back to back."""
 import os
+import subprocess
+import sys
 import threading
 
 import pytest
 import torch
 
 import gpu_mode_kernels_b200 as pkg
-from gpu_mode_kernels_b200 import _lib, linear as linear_module, moe
+from gpu_mode_kernels_b200 import _lib
 from gpu_mode_kernels_b200.all2all import A2AContext
 from gpu_mode_kernels_b200.linear import check, linear
 from gpu_mode_kernels_b200.local_world import LocalWorld
@@ -113,6 +115,78 @@ def test_experts_between_dispatch_and_combine(world, payload, T, routing, dtype)
     finally:
         group.close()
     check()
+
+
+@pytest.mark.gpu
+def test_experts_on_rows_that_came_as_fp8():
+    """Rows of -1, 0 and 1 are themselves after eight bits with a scale for 128 values, so the layer is the one of 16-bit rows."""
+    world, E, k, hidden, inner, T = 2, 8, 2, 256, 64, 17
+    w = Weights(3, E, hidden, inner).to(DEV)
+    datas = [pkg.generate_input(E, k, hidden, T, seed=72, rank=r, world_size=world) for r in range(world)]
+    rds = [d[1].to(DEV) for d in datas]
+    for rd in rds:
+        rd.x = rd.x.sign()
+    L, outs = E // world, []
+    for payload in ("fp8", "direct"):
+        group = LocalWorld(datas[0][0], world, payload=payload)
+        try:
+            outs.append(group.forward_phases(rds, experts=[(w.gate_up[r * L:(r + 1) * L], w.down[r * L:(r + 1) * L]) for r in range(world)]))
+            torch.cuda.synchronize()
+            group.check()
+        finally:
+            group.close()
+    assert all(torch.equal(bits(a), bits(b)) for a, b in zip(*outs))
+
+
+@pytest.mark.gpu
+def test_weights_written_just_before_the_call():
+    """The second product has its first weights on their way before the first one is through: what the stream did before counts."""
+    w = Weights(21, 16, 128, 64).to(DEV)
+    g = torch.Generator().manual_seed(22)
+    downs = [normal(g, 16, 128, 64).to(DEV) for _ in range(3)]
+    down = downs[0].clone()
+    for tokens in (1, 7, 90):
+        x = normal(g, tokens, 128).to(DEV)
+        idx, weights = route(x, w.router, 3)
+        want = [moe_layer(x, idx, weights, w.gate_up, d) for d in downs]
+        rows = normal(g, 16, 1, 40, 128).to(DEV)
+        counts = torch.full((1, 4, 16), 33, dtype=torch.int32, device=DEV)
+        slabs = [expert_mlp(rows, counts, w.gate_up, d, out=torch.zeros_like(rows)) for d in downs]
+        torch.cuda.synchronize()
+        got, on_slabs = [], []
+        for i in range(30):
+            down.copy_(downs[i % 3])
+            got.append(moe_layer(x, idx, weights, w.gate_up, down))
+            down.copy_(downs[(i + 1) % 3])
+            on_slabs.append(expert_mlp(rows, counts, w.gate_up, down, out=torch.zeros_like(rows)))
+        assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(got))
+        assert all(torch.equal(y, slabs[(i + 1) % 3]) for i, y in enumerate(on_slabs))
+
+
+@pytest.mark.gpu
+def test_a_first_call_may_be_a_captured_one():
+    """Nothing of a call's set-up, which the first one of a process makes, is forbidden in a capture."""
+    code = """
+import torch
+from gpu_mode_kernels_b200.linear import linear
+from gpu_mode_kernels_b200.moe import moe_layer, topk_gate, expert_mlp
+x, up, down = (torch.randn(*s, device="cuda").bfloat16() for s in ((80, 64), (8, 64, 64), (8, 64, 32)))
+idx, w = torch.zeros(80, 2, dtype=torch.int32, device="cuda"), torch.ones(80, 2, device="cuda")
+rows, counts = torch.randn(8, 1, 16, 64, device="cuda").bfloat16(), torch.full((1, 4, 8), 9, dtype=torch.int32, device="cuda")
+s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+def calls():
+    return [linear(x, up[0]), linear(x.repeat(30, 1), up[0]), linear(x[:2], up[0]), *topk_gate(x.float()[:, :8].contiguous(), 2, bias=w[:4].flatten()),
+            moe_layer(x, idx, w, up, down), moe_layer(x[:3], idx[:3], w[:3], up, down), expert_mlp(rows, counts, up, down, out=torch.zeros_like(rows))]
+with torch.cuda.graph(g, stream=s):
+    got = calls()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+print("alike")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0 and "alike" in done.stdout, done.stderr[-2000:]
 
 
 @pytest.mark.gpu

@@ -60,11 +60,11 @@ def experts_args(**kw):
 
 @pytest.mark.parametrize("make,entry,kw", [
     *[(gate_args, "a2a_gate", kw) for kw in (
-        dict(dtype=3), dict(experts=0), dict(experts=1025), dict(topk=0), dict(topk=9), dict(topk=33, experts=64), dict(score=2), dict(tokens=-1),
+        dict(dtype=3), dict(experts=0), dict(experts=1025), dict(topk=0), dict(topk=9), dict(topk=33, experts=64), dict(score=2), dict(tokens=-1), dict(tokens=(1 << 30) + 1),
         dict(logits=0), dict(indices=0), dict(weights=0), dict(stride=-8))],
     *[(linear_args, "a2a_linear", kw) for kw in (
         dict(dtype=2), dict(dtype=1, out_dtype=0), dict(bias=ONE, bias_dtype=1), dict(activation=5), dict(activation=-1), dict(tokens=-1),
-        dict(inputs=0), dict(inputs=60, x_stride=64), dict(outputs=0), dict(outputs=65537, y_stride=65537), dict(inputs=65544, x_stride=65544, weight_stride=65544),
+        dict(inputs=0), dict(inputs=60, x_stride=64), dict(outputs=0), dict(outputs=(1 << 24) + 1, y_stride=(1 << 24) + 1), dict(tokens=(1 << 30) + 1), dict(inputs=65544, x_stride=65544, weight_stride=65544),
         dict(x=0), dict(weight=0), dict(y=0), dict(x=ONE + 8), dict(weight=ONE + 2), dict(x_stride=56), dict(x_stride=68), dict(weight_stride=60),
         dict(y_stride=15), dict(residual=ONE, residual_stride=-1))],
     *[(layer_args, "a2a_layer", kw) for kw in (
@@ -232,6 +232,20 @@ def test_linear_epilogues(tokens, activation, bias, residual, out):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,inputs,outputs", [(2000, 512, 1100), (1100, 136, 2048), (513, 1024, 2050), (1030, 2048, 384), (90, 2880, 700)])
+@pytest.mark.parametrize("activation,bias,residual,out", [("none", None, True, None), ("swiglu", "fp32", True, torch.float32), ("gelu", "same", False, None),
+                                                          ("swiglu", None, False, None), ("silu", "same", True, torch.float32)])
+def test_linear_many_rows(tokens, inputs, outputs, activation, bias, residual, out):
+    """Single blocks, clusters that share a sum and pairs of blocks; whole and ragged tiles; stores of sixteen bytes and of single values."""
+    g, dtype = generator(tokens, activation), torch.bfloat16 if outputs % 4 else torch.float16
+    rows = outputs * (2 if activation == "swiglu" else 1)
+    b = None if bias is None else normal(g, rows, dtype=dtype if bias == "same" else torch.float32)
+    check_linear(normal(g, tokens, inputs, dtype=dtype), normal(g, rows, inputs, std=inputs ** -0.5, dtype=dtype), b, activation,
+                 normal(g, tokens, outputs, dtype=out or dtype) if residual else None, out)
+    check()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens,inputs,outputs", [(1, 7168, 600), (16, 7168, 256), (64, 7168, 256), (40, 4096, 1000), (3, 20000, 40)])
 def test_linear_long_sums(tokens, inputs, outputs):
     g = generator(tokens, inputs)
@@ -250,6 +264,8 @@ def test_linear_strides_shapes_and_views():
         check_linear(base[:rows:2, 3:259], w[:, :256])              # a start that is off 16 bytes: copied
         check_linear(base.t()[:rows, :80], w[::2, :80])             # columns for rows: copied
         check_linear(base[:1, :256].expand(rows, 256), w[:, :256])  # one row many times
+        shifted = torch.empty(rows * 256 + 3, dtype=torch.bfloat16, device=DEV)[3:].view(rows, 256).copy_(base[:rows, :256])
+        check_linear(shifted, w[:, :256].contiguous())              # contiguous, but off 16 bytes: copied
         check_linear(base[:rows, :256], w[:, :256], residual=base[:rows, 100:196])
         check_linear(base[:rows, :256], w[:, :256], residual=base[:1, 100:196].expand(rows, 96))
         check_linear(base[:rows, :256], w[:, :256], residual=normal(g, 96, rows, dtype=torch.bfloat16).to(DEV).t())
@@ -258,6 +274,16 @@ def test_linear_strides_shapes_and_views():
     check_linear(base[:1, :64], w[:1, :64])
     assert linear(base[:0, :64], w[:, :64]).shape == (0, 96)
     assert linear(base.view(4, 20, 400)[:, :0, :64], w[:, :64]).shape == (4, 0, 96)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 30, 300])
+def test_linear_many_outputs(tokens):
+    """As many as a vocabulary has, past the sizes that a layer's matrices have."""
+    g = generator(tokens, 70001)
+    x, w = normal(g, tokens, 64, dtype=torch.bfloat16), normal(g, 70001, 64, std=0.125, dtype=torch.bfloat16)
+    check_linear(x, w, out_dtype=torch.float32)
+    check_linear(x, w, normal(g, 70001, dtype=torch.bfloat16), residual=normal(g, tokens, 70001, dtype=torch.bfloat16))
 
 
 @pytest.mark.gpu
