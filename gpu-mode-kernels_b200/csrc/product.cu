@@ -161,7 +161,10 @@ DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
         const int columns = round16(parts_of(a.tokens, across));
         const float tail = columns * 13.0f;
         auto consider = [&](int down, int split) {
-            const int height = parts_of(a.outputs, down), tiles = parts_of(a.outputs, height) * across;
+            int height = parts_of(a.outputs, down);
+            if (columns > 16 && most % 8 == 0) height = (height + 7) & ~7;  // stores of sixteen bytes
+            const int tiles = parts_of(a.outputs, height) * across;
+            if (split > 1 && tiles > most_clusters<kDense, T, false>(split)) return;
             const int busy = std::min(tiles * split, sms), rounds = split > 1 ? 1 : parts_of(tiles, sms);
             const float block = block_ns(paired ? 2 * height : height, columns, columns, busy / (6500.0f * across));
             const float t = rounds * parts_of(blocks, split) * std::max(block, 1.3f * std::min(parts_of(a.outputs, height), sms)) + tail +
