@@ -11,6 +11,11 @@ Public surface (mirrors the reference task, amd-distributed/all2all):
 * ``A2AContext`` -- per-process-group state: symmetric receive buffers, peer
   mappings, flags (the role ``P2PState`` plays in submission_v9.py:880-947).
 
+* ``moe`` and ``linear`` -- the layer around it: the gate that chooses the experts
+  (``moe.topk_gate``), the experts on one GPU or between dispatch and combine
+  (``moe.moe_layer``, ``A2AContext.experts``), dense products with an epilogue
+  (``linear.linear``).
+
 Importing this package does not load the CUDA library; the first use of
 ``A2AContext`` / ``custom_kernel`` does, and raises if it is missing.
 """

@@ -108,7 +108,6 @@ int most_clusters(int size) {
             return 0;
         }
         known[size].store(++n, std::memory_order_relaxed);
-
     }
     return n - 1;
 }
