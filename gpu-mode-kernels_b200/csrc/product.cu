@@ -275,8 +275,8 @@ int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
     return launch(reinterpret_cast<const void*>(&layer_sum_kernel<T>), dim3(a.tokens, parts_of(a.hidden_dim, 4 * kSumThreads)), kSumThreads, 0, 1, &sum, st);
 }
 
-// Rows of inner values that a call on slabs may have: those of a slab are rounded up to whole boxes of eight.
-long long inner_rows(int local_experts, int world, int capacity) { return (long long)local_experts * world * ((capacity + 7) & ~7); }
+// Rows of inner values that a call on slabs may have: those of a slab are rounded up to whole steps.
+long long inner_rows(int local_experts, int world, int capacity) { return (long long)local_experts * world * ((capacity + kManyStep - 1) & -kManyStep); }
 
 template <typename T>
 int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {

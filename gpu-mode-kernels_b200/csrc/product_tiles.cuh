@@ -51,6 +51,7 @@ constexpr int kTmemColumns = 512;
 constexpr int kSpreadTokens = 64;  // 40 to 100 tokens take the same either way
 constexpr int kPieceRows = 32;  // operand rows of a box of a tile that is less than full
 constexpr int kMaxSplit = 8;
+constexpr int kManyStep = 32;  // columns of a source in the slabs come in so many where there are many
 constexpr int kCached = 4096;  // pairs whose experts a block keeps in shared memory
 
 struct TilesParams {
@@ -194,15 +195,18 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         cudaTriggerProgrammaticLaunchCompletion();
     }
 
+    // kSlab*: rows that source `src` has for group g, and the columns of a group, with those of every source rounded up to whole steps
+    auto slab_rows = [&](int g, int src) { return min(max(p.counts[(size_t)src * 4 * p.groups + g], 0), p.capacity); };
+    auto slab_columns = [&](int g, int step) {
+        int n = 0;
+        for (int src = 0; src < p.world; ++src) n += (slab_rows(g, src) + step - 1) & -step;
+        return n;
+    };
+
     // ---- how many columns every group has, and so the tiles ----
-    int columns = p.columns, height = p.full;
+    int columns = p.columns, height = p.full, slab_step = 8;
     if (kGrouped) {
-        for (int g = tid; g < p.groups; g += kTilesThreads) {
-            int n = 0;
-            if (kSlab)  // a rank's rows in whole boxes of eight
-                for (int src = 0; src < p.world; ++src) n += (min(max(p.counts[(size_t)src * 4 * p.groups + g], 0), p.capacity) + 7) & ~7;
-            s.count[g] = n;
-        }
+        for (int g = tid; g < p.groups; g += kTilesThreads) s.count[g] = kSlab ? slab_columns(g, 8) : 0;
         __syncthreads();
         if (kLayer) {
             for (int i = tid; i < p.tokens * p.topk; i += kTilesThreads) {
@@ -218,6 +222,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0) atomicMax(&s.largest, most);
         __syncthreads();
+        if (kSlab && s.largest > kMaxColumns) {
+            // more than a tile of columns: columns without a row cost less than boxes of eight
+            slab_step = kManyStep;
+            for (int g = tid; g < p.groups; g += kTilesThreads) s.count[g] = slab_columns(g, slab_step);
+            __syncthreads();
+        }
         columns = min(p.columns, (max(s.largest, 1) + kColumnStep - 1) / kColumnStep * kColumnStep);
         if (warp == 0) {
             int run = 0, rows = 0;
@@ -308,7 +318,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         const int across = parts_of(count, columns);
         const int m = quotient(t, across);
         x.f = kBlocks * (m * height + cut) + side * x.height;  // this block's
-
         x.first = (t - m * across) * columns;
         x.columns = min(columns, count - x.first);
         return x;
@@ -487,23 +496,29 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                         for (int c = lane; c < x.columns; c += 32) s.scale[buffer][c] = p.weights_of[s.list[buffer][c]];
                     }
                 } else {
-                    for (int c = lane; c < x.columns; c += 32) {
+                    // the row of the slabs that stands at a column, and whether it is a valid one
+                    auto row_at = [&](int c, bool& valid) {
                         int r = x.first + c, src = 0, have = 0;
-                        for (; src < p.world; ++src) {
-                            have = min(max(p.counts[(size_t)src * 4 * p.groups + x.group], 0), p.capacity);
-                            const int room = (have + 7) & ~7;
+                        for (; src < p.world - 1; ++src) {
+                            have = slab_rows(x.group, src);
+                            const int room = (have + slab_step - 1) & -slab_step;
                             if (r < room) break;
                             r -= room;
                         }
-                        s.list[buffer][c] = src < p.world && r < have ? (x.group * p.world + src) * p.capacity + r : -1;
+                        if (src == p.world - 1) have = slab_rows(x.group, src);
+                        valid = r < have;
+                        return (x.group * p.world + src) * p.capacity + r;
+                    };
+                    bool valid;
+                    for (int c = lane; c < x.columns; c += 32) {
+                        const int row = row_at(c, valid);
+                        s.list[buffer][c] = valid ? row : -1;
                     }
-                    __syncwarp();
-                    // Every eight columns begin with a row; lane i looks at columns 8 i to 8 i + 7, where its run begins and ends, and
-                    // whether a box begins there.
+                    // Lane i looks at columns 8 i to 8 i + 7: where their run begins and ends, and whether a box begins there.
                     int box_rows = 0;
                     for (int of = 0; of < kBlocks; ++of) {
                         int from;
-                        const int eights = columns_of(x, of, from) >> 3, row = lane < eights ? s.list[buffer][from + 8 * lane] : -1;
+                        const int eights = columns_of(x, of, from) >> 3, row = lane < eights ? row_at(from + 8 * lane, valid) : -1;
                         const int before = __shfl_up_sync(0xffffffffu, row, 1);
                         const unsigned breaks = __ballot_sync(0xffffffffu, lane == 0 || lane >= eights || row != before + 8);
                         const int run0 = 31 - __clz(breaks & (0xffffffffu >> (31 - lane)));
