@@ -100,13 +100,19 @@ __device__ __forceinline__ void exchange_eight(float (&v)[8], int lane) {
 // (The quick division gives 0 where the divisor is above 2^126: below -87, where silu is less than 1e-35.)
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + expf(-v)); }
 
-__device__ __forceinline__ float activate(float v, int activation) {
-    switch (activation) {
-        // relu passes a NaN on, as torch's does
-        case A2A_ACT_RELU: return v < 0.0f ? 0.0f : v;
-        case A2A_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-        case A2A_ACT_SILU: return silu(v);
-        default: return v;
+// Over all values at once: the choice inside a loop over them was two thirds of the epilogue (16384 rows of 1024 to 2048: 92 us where this takes
+// 62).
+template <int kCount>
+__device__ __forceinline__ void activate(float (&v)[kCount], int activation) {
+    if (activation == A2A_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];  // passes a NaN on, as torch's does
+    } else if (activation == A2A_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) v[j] = 0.5f * v[j] * (1.0f + erff(v[j] * 0.70710678118654752f));
+    } else if (activation == A2A_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) v[j] = silu(v[j]);
     }
 }
 

@@ -603,18 +603,18 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 }
                 if (!inside) return;
                 if (kOp == kDense) {
-                    float add[kCount];
+                    float add[kCount], out[kCount];
 #pragma unroll
                     for (int j = 0; j < kCount; ++j) {
                         add[j] = 0.0f;
                         if (p.residual != nullptr && c0 + j < x.columns)
                             add[j] = load_any<T>(p.residual, (size_t)(x.first + c0 + j) * p.residual_stride + f, p.out_fp32);
+                        out[j] = v[j] + bias;
                     }
-#pragma unroll
-                    for (int j = 0; j < kCount; ++j) add[j] += activate(v[j] + bias, p.activation);
+                    activate(out, p.activation);
 #pragma unroll
                     for (int j = 0; j < kCount; ++j)
-                        if (c0 + j < x.columns) store_any<T>(p.y, (size_t)(x.first + c0 + j) * p.y_stride + f, add[j], p.out_fp32);
+                        if (c0 + j < x.columns) store_any<T>(p.y, (size_t)(x.first + c0 + j) * p.y_stride + f, out[j] + add[j], p.out_fp32);
                 } else {
 #pragma unroll
                     for (int j = 0; j < kCount; ++j) {
@@ -678,7 +678,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 for (int h = 0; h < 2 && !paired; ++h) {
                     float out[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) out[j] = kOp == kDense ? activate(v[8 * h + j] + bias, p.activation) : v[8 * h + j];
+                    for (int j = 0; j < 8; ++j) out[j] = kOp == kDense ? v[8 * h + j] + bias : v[8 * h + j];
+                    if (kOp == kDense) activate(out, p.activation);
                     exchange_eight<1>(out, lane);
                     store_eight(out, c0 + 8 * h + (lane & 7), quarter * 32 + 8 * (lane >> 3));
                 }
