@@ -96,6 +96,32 @@ __device__ __forceinline__ void exchange_eight(float (&v)[8], int lane) {
     }
 }
 
+// The same for values that are rounded to 16 bits anyway: the second and third exchange are of two values at a time.
+template <int kStep, typename T>
+__device__ __forceinline__ uint4 exchange_packed(float (&v)[8], int lane) {
+    const bool high = lane & kStep;
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float got = __shfl_xor_sync(0xffffffffu, high ? v[i] : v[i + 1], kStep);
+        alignas(4) T two[2] = {Element<T>::from_float(high ? got : v[i]), Element<T>::from_float(high ? v[i + 1] : got)};
+        q[i / 2] = *reinterpret_cast<const uint32_t*>(two);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const bool up = lane & 2 * kStep << k;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i >> k & 1) continue;
+            const int j = i | 1 << k;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? q[i] : q[j], 2 * kStep << k);
+            q[i] = up ? got : q[i];
+            q[j] = up ? q[j] : got;
+        }
+    }
+    return make_uint4(q[0], q[1], q[2], q[3]);
+}
+
 // ---- the epilogue's arithmetic: fp32, on the fp32 sums of a product -------------------------------
 // (The quick division gives 0 where the divisor is above 2^126: below -87, where silu is less than 1e-35.)
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + expf(-v)); }

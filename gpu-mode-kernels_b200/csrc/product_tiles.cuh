@@ -98,6 +98,11 @@ __host__ __device__ __forceinline__ int quotient(int a, int b) {
 }
 __host__ __device__ __forceinline__ int parts_of(int n, int size) { return quotient(n + size - 1, size); }
 
+template <int kNumber>
+struct Lanes {
+    static constexpr int value = kNumber;
+};
+
 // How `tiles` tiles of `height` features go over `blocks` blocks: whole rounds, and those of the last round in `cut` parts of `part` features.
 struct Rounds {
     int whole, cut, part;
@@ -630,37 +635,59 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             // feature into 8 features of a column. (A store of two bytes for each value: 132 us for experts on slabs of 7000 rows of 2048
             // where this takes 117.)
             const bool wide_stores = kOp != kLayerDown && p.wide_stores && (x.f & 7) == 0 && (x.height & 7) == 0;
-            auto store_eight = [&](float (&v)[8], int c, int within8) {
-                const int f0 = x.f + within8;
-                if (within8 >= x.height || f0 >= p.features || c >= x.columns) return;
-                size_t o;
-                void* to;
-                bool fp32 = false;
+            // where features f0 to f0 + 7 of column c go, and how many of them there are; none: 0
+            auto place_of = [&](int c, int within8, int& f0, void*& to, size_t& o) {
+                f0 = x.f + within8;
+                if (within8 >= x.height || f0 >= p.features || c >= x.columns) return 0;
                 if (kOp == kDense) {
-                    const size_t token = x.first + c;
-                    fp32 = p.out_fp32;
-                    o = token * p.y_stride + f0;
+                    o = (size_t)(x.first + c) * p.y_stride + f0;
                     to = p.y;
-                    if (f0 + 8 > p.features) {  // the last ones, not eight
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (f0 + j >= p.features) break;
-                            const float add = p.residual != nullptr ? load_any<T>(p.residual, token * p.residual_stride + f0 + j, fp32) : 0.0f;
-                            store_any<T>(to, o + j, v[j] + add, fp32);
-                        }
-                        return;
-                    }
-                    if (p.residual != nullptr) add_eight<T>(v, p.residual, token * p.residual_stride + f0, fp32);
-                } else if (kUp) {
-                    // Rounded to the rows' type, since the next product takes 16-bit operands.
+                    return min(8, p.features - f0);
+                }
+                if (kUp) {
                     o = (size_t)(s.row[x.group] + x.first + c) * p.features + f0;
                     to = p.hidden;
-                } else {
-                    if (s.list[buffer][c] < 0) return;
-                    o = (size_t)s.list[buffer][c] * p.features + f0;
-                    to = p.y;
+                    return 8;
                 }
-                put_eight<T>(to, o, v, fp32);
+                const int row = s.list[buffer][c];
+                o = (size_t)row * p.features + f0;
+                to = p.y;
+                return row >= 0 ? 8 : 0;
+            };
+            // kStep: what the columns of the eight values differ by in lanes. Inner values are rounded to the rows' type, since the next product
+            // takes 16-bit operands.
+            auto store_eight = [&](float (&v)[8], auto step, int c, int within8) {
+                constexpr int kStep = decltype(step)::value;
+                int f0;
+                void* to;
+                size_t o;
+                if (kOp != kDense || (p.residual == nullptr && !p.out_fp32)) {
+                    const uint4 q = exchange_packed<kStep, T>(v, lane);
+                    const int n = place_of(c, within8, f0, to, o);
+                    if (n == 8) {
+                        *reinterpret_cast<uint4*>(static_cast<T*>(to) + o) = q;
+                    } else if (n > 0) {  // the last ones
+                        const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (j < n) reinterpret_cast<uint16_t*>(to)[o + j] = (uint16_t)(word[j / 2] >> 16 * (j & 1));
+                    }
+                    return;
+                }
+                exchange_eight<kStep>(v, lane);
+                const int n = place_of(c, within8, f0, to, o);
+                const size_t from = (size_t)(x.first + c) * p.residual_stride + f0;
+                if (n == 8) {
+                    if (p.residual != nullptr) add_eight<T>(v, p.residual, from, p.out_fp32);
+                    put_eight<T>(to, o, v, p.out_fp32);
+                } else if (n > 0) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (j >= n) break;
+                        const float add = p.residual != nullptr ? load_any<T>(p.residual, from + j, p.out_fp32) : 0.0f;
+                        store_any<T>(to, o + j, v[j] + add, p.out_fp32);
+                    }
+                }
             };
             auto finish_wide = [&](int c0, float (&v)[16]) {
                 if (paired) {
@@ -671,8 +698,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                         const float other = __shfl_xor_sync(0xffffffffu, up ? even : odd, 1);
                         out[j] = silu(up ? other : even) * (up ? odd : other);
                     }
-                    exchange_eight<2>(out, lane);
-                    store_eight(out, c0 + (lane & 15), quarter * 16 + 8 * (lane >> 4));
+                    store_eight(out, Lanes<2>(), c0 + (lane & 15), quarter * 16 + 8 * (lane >> 4));
                 }
 #pragma unroll
                 for (int h = 0; h < 2 && !paired; ++h) {
@@ -680,8 +706,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
 #pragma unroll
                     for (int j = 0; j < 8; ++j) out[j] = kOp == kDense ? v[8 * h + j] + bias : v[8 * h + j];
                     if (kOp == kDense) activate(out, p.activation);
-                    exchange_eight<1>(out, lane);
-                    store_eight(out, c0 + 8 * h + (lane & 7), quarter * 32 + 8 * (lane >> 3));
+                    store_eight(out, Lanes<1>(), c0 + 8 * h + (lane & 7), quarter * 32 + 8 * (lane >> 3));
                 }
             };
             if (kOp == kDense && !kPair && split > 1) {
