@@ -148,13 +148,15 @@ struct DensePlan {
 // addition takes 1.5 us and 10 ns a column, the epilogue of the last tile 13 ns a column, and blocks that read the same rows at the same
 // time 1.3 ns each. (With 256 columns wherever there are as many: 1024 rows of
 // 2048 to 2048 27.6 us instead of 14.9, 200 of 4096 to 7168 30.8 instead of 22.7.)
-template <typename T>
+template <TilesOp kOp, typename T>
 DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
     const int most = std::min(paired ? kTileRows / 2 : kTileRows, a.outputs), blocks = parts_of(a.inputs, kTileInner), least_down = parts_of(a.outputs, most);
-    DensePlan best{most, std::min(kMaxColumns, round16(a.tokens)), 1, false};
+    constexpr int widest = kOp == kDense32 ? kMaxColumns32 : kMaxColumns;
+    DensePlan best{most, std::min(widest, round16(a.tokens)), 1, false};
     float least = 1e30f;
     static constexpr int kWidths[] = {256, 192, 160, 128, 96, 64, 48, 32, 16};
     for (const int width : kWidths) {
+        if (width > widest) continue;
         const int across = parts_of(a.tokens, width);
         if (width > 16 && across == parts_of(a.tokens, width - 16) && width - 16 >= a.tokens) continue;  // wider than all there is
         const int columns = round16(parts_of(a.tokens, across));
@@ -163,7 +165,7 @@ DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
             int height = parts_of(a.outputs, down);
             if (columns > 16 && most % 8 == 0) height = (height + 7) & ~7;  // stores of sixteen bytes
             const int tiles = parts_of(a.outputs, height) * across;
-            if (split > 1 && tiles > most_clusters<kDense, T, false>(split)) return;
+            if (split > 1 && tiles > most_clusters<kOp, T, false>(split)) return;
             const int busy = std::min(tiles * split, sms), rounds = split > 1 ? 1 : parts_of(tiles, sms);
             const float block = block_ns(paired ? 2 * height : height, columns, columns, busy / (6500.0f * across));
             const float t = rounds * parts_of(blocks, split) * std::max(block, 1.3f * std::min(parts_of(a.outputs, height), sms)) + tail +
@@ -176,13 +178,13 @@ DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
             if (down > least_down && parts_of(a.outputs, down) >= std::min(most, 8)) consider(down, 1);
         }
         for (int split = 2; split <= std::min(kMaxSplit, blocks); ++split) {
-            const int room = most_clusters<kDense, T, false>(split), down = room / across;
+            const int room = most_clusters<kOp, T, false>(split), down = room / across;
             if (down < least_down) break;
             consider(least_down, split);
             if (down > least_down && parts_of(a.outputs, down) >= std::min(most, 8)) consider(down, split);
         }
         if (width % 32 == 0) {
-            const int wide = (parts_of(a.tokens, across) + 31) / 32 * 32, tiles = parts_of(a.outputs, 2 * most) * across, units = most_clusters<kDense, T, true>(2);
+            const int wide = (parts_of(a.tokens, across) + 31) / 32 * 32, tiles = parts_of(a.outputs, 2 * most) * across, units = most_clusters<kOp, T, true>(2);
             if (units < 1) continue;
             const float t = parts_of(tiles, units) * blocks * block_ns(paired ? 2 * most : most, wide, wide / 2, 2 * std::min(tiles, units) / (6500.0f * across)) + tail;
             if (t < least * 0.999f) least = t, best = DensePlan{most, wide, 1, true};
@@ -193,25 +195,25 @@ DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-template <typename T>
+template <TilesOp kOp, typename T>
 int linear_of(const a2a_linear_args& a, int sms, cudaStream_t st) {
     const bool paired = a.activation == A2A_ACT_SWIGLU;
     TilesParams p{};
     p.inner = a.inputs, p.features = a.outputs, p.paired = paired, p.groups = 1, p.tokens = a.tokens;
-    p.activation = a.activation, p.out_fp32 = a.out_dtype == A2A_DTYPE_FP32, p.bias_fp32 = a.bias_dtype == A2A_DTYPE_FP32;
+    p.activation = a.activation, p.bias_fp32 = a.bias_dtype == A2A_DTYPE_FP32;
     p.bias = a.bias, p.residual = a.residual, p.residual_stride = a.residual_stride, p.y = a.y, p.y_stride = a.y_stride;
     p.wide_stores = a.y_stride % 8 == 0 && aligned(a.y) && (a.residual == nullptr || (a.residual_stride % 8 == 0 && aligned(a.residual)));
-    const DensePlan plan = dense_plan<T>(a, paired, sms);
+    const DensePlan plan = dense_plan<kOp, T>(a, paired, sms);
     p.columns = plan.columns, p.full = plan.height, p.split = plan.split;
     int rc = weights_map(&p.weights, a.dtype, a.weight, 1, a.outputs, paired, a.inputs, a.weight_stride, plan.height);
     if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.inputs, a.x_stride, plan.pair ? p.columns / 2 : p.columns);
     if (rc != A2A_OK) return rc;
     if (plan.pair) {
         const int tiles = parts_of(a.outputs, 2 * plan.height) * parts_of(a.tokens, plan.columns);
-        return launch_tiles<kDense, T, true>(p, 2 * std::min(tiles, most_clusters<kDense, T, true>(2)), 2, st);
+        return launch_tiles<kOp, T, true>(p, 2 * std::min(tiles, most_clusters<kOp, T, true>(2)), 2, st);
     }
     const int tiles = parts_of(a.outputs, plan.height) * parts_of(a.tokens, plan.columns);
-    return launch_tiles<kDense, T>(p, plan.split > 1 ? tiles * plan.split : std::min(tiles, sms), plan.split, st);
+    return launch_tiles<kOp, T>(p, plan.split > 1 ? tiles * plan.split : std::min(tiles, sms), plan.split, st);
 }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -314,7 +316,9 @@ extern "C" int a2a_linear(const a2a_linear_args* args, void* stream) {
     const int rc = sm_count(&sms);
     if (rc != A2A_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    return a.dtype == A2A_DTYPE_BF16 ? linear_of<__nv_bfloat16>(a, sms, st) : linear_of<__half>(a, sms, st);
+    if (a.out_dtype == A2A_DTYPE_FP32)
+        return a.dtype == A2A_DTYPE_BF16 ? linear_of<kDense32, __nv_bfloat16>(a, sms, st) : linear_of<kDense32, __half>(a, sms, st);
+    return a.dtype == A2A_DTYPE_BF16 ? linear_of<kDense, __nv_bfloat16>(a, sms, st) : linear_of<kDense, __half>(a, sms, st);
 }
 
 extern "C" size_t a2a_layer_workspace(int num_tokens, int experts_per_token, int hidden_dim, int inner) {

@@ -37,7 +37,8 @@
 
 namespace {
 
-enum TilesOp { kDense, kLayerUp, kLayerDown, kSlabUp, kSlabDown };
+// kDense32: with a result of 32 bits
+enum TilesOp { kDense, kDense32, kLayerUp, kLayerDown, kSlabUp, kSlabDown };
 
 constexpr int kTileRows = 128, kTileInner = 64, kMaxColumns = 256;
 constexpr int kRowBytes = kTileInner * 2;
@@ -51,6 +52,11 @@ constexpr int kTmemColumns = 512;
 constexpr int kSpreadTokens = 64;  // 40 to 100 tokens take the same either way
 constexpr int kPieceRows = 32;  // operand rows of a box of a tile that is less than full
 constexpr int kMaxSplit = 8;
+// The tensor core cuts the sums it adds to: a sum of 7168 products came out 8e-6 off, of the 2-norm, where fp32 additions are 9e-7 off. For a result
+// of 32 bits a sum in tensor memory therefore is of about 512 of the inner length (5e-7 off), and the epilogue's threads add the parts up in
+// registers, which hold 128 columns. A sum of up to 896 is left whole (9e-7; 256 outputs of 7168, 16 rows, 6.5 us in parts and 5.9 at once), but for
+// SwiGLU, whose product doubles the error.
+constexpr int kSumBlocks = 8, kSumBlocksAtOnce = 14, kMaxColumns32 = 128;
 constexpr int kManyStep = 32;  // columns of a source in the slabs come in so many where there are many
 constexpr int kCached = 4096;  // pairs whose experts a block keeps in shared memory
 
@@ -68,7 +74,7 @@ struct TilesParams {
     int split;                  // kDense: blocks of a cluster, which share a tile's inner length
     int tokens;
     // kDense: the epilogue
-    int activation, out_fp32, bias_fp32;
+    int activation, bias_fp32;
     int wide_stores;  // rows of y, and of the residual, begin on 16 bytes
     const void* bias;
     const void* residual;
@@ -148,6 +154,28 @@ static_assert(sizeof(TilesShared) >= kTileRows * kRowBytes, "operands of 128 row
 constexpr size_t kTilesSharedBytes = 1024 + kRingBytes + sizeof(TilesShared);
 static_assert(kTilesSharedBytes <= 227 * 1024, "a block's shared memory");
 
+// The epilogue's 16 columns from 16 * half on, in steps of 32, with the registers that hold them (kParts: one for results of 16 bits).
+template <int kParts, typename Do>
+__device__ __forceinline__ void for_parts(int columns, int half, float (&total)[kParts][16], Do work) {
+    if constexpr (kParts > 1) {
+#pragma unroll
+        for (int g = 0; g < kParts; ++g)
+            if (16 * half + 32 * g < columns) work(16 * half + 32 * g, total[g]);
+    } else {
+        for (int c0 = 16 * half; c0 < columns; c0 += 32) work(c0, total[0]);
+    }
+}
+template <int kParts>
+__device__ __forceinline__ void add_part(uint32_t sums, bool needed, int columns, int half, float (&total)[kParts][16]) {
+    if (!needed) return;
+    for_parts(columns, half, total, [&](int c0, float (&sum)[16]) {
+        float v[16];
+        tmem_load_16(sums + c0, v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[j] += v[j];
+    });
+}
+
 struct Tile {
     int group, f, height, first, columns;  // matrix, first feature, features, first column, columns
 };
@@ -164,15 +192,15 @@ __host__ __device__ __forceinline__ float block_ns(int rows, int columns, int he
 
 template <TilesOp kOp, typename T, bool kPair>
 __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const __grid_constant__ TilesParams p) {
-    constexpr bool kGrouped = kOp != kDense, kLayer = kOp == kLayerUp || kOp == kLayerDown, kSlab = kOp == kSlabUp || kOp == kSlabDown;
+    constexpr bool k32 = kOp == kDense32, kOne = kOp == kDense || k32, kGrouped = !kOne, kLayer = kOp == kLayerUp || kOp == kLayerDown, kSlab = kOp == kSlabUp || kOp == kSlabDown;
     constexpr bool kUp = kOp == kLayerUp || kOp == kSlabUp;
-    const bool first = kOp == kDense || (kOp == kLayerUp && !p.sorted) || kOp == kSlabUp;  // nothing of the same call runs before it
+    const bool first = kOne || (kOp == kLayerUp && !p.sorted) || kOp == kSlabUp;  // nothing of the same call runs before it
     const bool runs = kGrouped && (!kUp || (kOp == kLayerUp && p.sorted));              // rows by expert
     extern __shared__ uint8_t shared_raw[];
     uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(shared_raw) + 1023) & ~(uintptr_t)1023);
     TilesShared& s = *reinterpret_cast<TilesShared*>(ring + kRingBytes);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const bool paired = kUp || (kOp == kDense && p.paired);
+    const bool paired = kUp || (kOne && p.paired);
     constexpr int kBlocks = kPair ? 2 : 1, kColumnStep = 16 * kBlocks;
     const int side = kPair ? (int)blockIdx.x & 1 : 0, units = (int)gridDim.x / kBlocks;  // block of the pair; blocks or pairs
 
@@ -290,7 +318,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     const int per_stage = min(blocks_all, max(1, quotient(kStageBytes + block_bytes / 2, block_bytes)));
     const int stages = min(kMaxStages, quotient(kRingBytes, block_bytes * per_stage));
     // this block's part of the inner length, and its tiles
-    const int split = kOp == kDense && !kPair ? p.split : 1, part = kOp == kDense && !kPair ? (int)blockIdx.x % split : 0;
+    const int split = kOne && !kPair ? p.split : 1, part = kOne && !kPair ? (int)blockIdx.x % split : 0;
     const int block0 = blocks_all * part / split, blocks = blocks_all * (part + 1) / split - block0;
     const int tile0 = (int)blockIdx.x / (kBlocks * split), tile_step = units / split;
 
@@ -329,7 +357,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     };
     // columns of a tile's product, and of those the ones that block `of` of the pair copies
     auto product_columns = [&](const Tile& x) {
-        if (kOp == kDense && kPair) return columns;
+        if (kOne && kPair) return columns;
         return ((kOp == kLayerUp && !p.sorted ? p.tokens : x.columns) + kColumnStep - 1) / kColumnStep * kColumnStep;
     };
     auto columns_of = [&](const Tile& x, int of, int& from) {
@@ -349,6 +377,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     };
     const bool spread = kOp == kLayerUp && !p.sorted;  // all tokens are a tile's columns
     const uint32_t stage_bytes = (uint32_t)per_stage * block_bytes;
+    // kDense32: of a sum in tensor memory, whole stages
+    const int sum_blocks = !paired && blocks <= kSumBlocksAtOnce ? blocks : max(1, kSumBlocks / per_stage) * per_stage;
     if (warp == 0) {
         if (elect_one()) {
             int stage = 0;
@@ -385,30 +415,35 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             int stage = 0, n = 0;
             uint32_t phase = 0;
             const uint64_t ring_descriptor = operand_descriptor(ring0);
-            for (int t = tile0; t < tiles; t += tile_step, ++n) {
+            for (int t = tile0; t < tiles; t += tile_step) {
                 const Tile x = tile_of(t);
-                const int buffer = n & 1;
                 const uint32_t descriptor = instruction_descriptor(Element<T>::kFormat, kTileRows * kBlocks, product_columns(x));
-                const uint32_t sums = tmem + buffer * kMaxColumns;
-                if (!barrier_wait(sums_empty0 + 8 * buffer, ((n >> 1) & 1) ^ 1, &s.gave_up)) goto products_done;
-                tcgen05_after_sync();
-                bool add = false;
-                for (int left = blocks; left > 0; left -= per_stage) {
-                    uint64_t w = ring_descriptor + (stage * stage_bytes >> 4);
-                    if (!barrier_wait(full0 + 8 * stage, phase, &s.gave_up)) goto products_done;
-                    for (int b = min(per_stage, left); b > 0; --b, w += block_bytes >> 4) {
-                        const uint64_t r = w + (weight_bytes >> 4);
-                        // 16 of the inner length are 32 bytes of a row
-                        tcgen05_mma<kPair>(sums, w, r, descriptor, add);
-                        tcgen05_mma<kPair>(sums, w + 2, r + 2, descriptor, true);
-                        tcgen05_mma<kPair>(sums, w + 4, r + 4, descriptor, true);
-                        tcgen05_mma<kPair>(sums, w + 6, r + 6, descriptor, true);
-                        add = true;
+                for (int chunk = blocks; chunk > 0; ++n) {
+                    // a sum in tensor memory: the whole inner length, or for a result of 32 bits a part of it
+                    const int buffer = n & 1;
+                    const uint32_t sums = tmem + buffer * kMaxColumns;
+                    if (!barrier_wait(sums_empty0 + 8 * buffer, ((n >> 1) & 1) ^ 1, &s.gave_up)) goto products_done;
+                    tcgen05_after_sync();
+                    bool add = false;
+                    const int end = k32 ? max(0, chunk - sum_blocks) : 0;
+                    for (int left = chunk; left > end; left -= per_stage) {
+                        uint64_t w = ring_descriptor + (stage * stage_bytes >> 4);
+                        if (!barrier_wait(full0 + 8 * stage, phase, &s.gave_up)) goto products_done;
+                        for (int b = min(per_stage, left); b > 0; --b, w += block_bytes >> 4) {
+                            const uint64_t r = w + (weight_bytes >> 4);
+                            // 16 of the inner length are 32 bytes of a row
+                            tcgen05_mma<kPair>(sums, w, r, descriptor, add);
+                            tcgen05_mma<kPair>(sums, w + 2, r + 2, descriptor, true);
+                            tcgen05_mma<kPair>(sums, w + 4, r + 4, descriptor, true);
+                            tcgen05_mma<kPair>(sums, w + 6, r + 6, descriptor, true);
+                            add = true;
+                        }
+                        tcgen05_commit<kPair>(empty0 + 8 * stage);
+                        if (++stage == stages) stage = 0, phase ^= 1;
                     }
-                    tcgen05_commit<kPair>(empty0 + 8 * stage);
-                    if (++stage == stages) stage = 0, phase ^= 1;
+                    tcgen05_commit<kPair>(sums_full0 + 8 * buffer);
+                    chunk = end;
                 }
-                tcgen05_commit<kPair>(sums_full0 + 8 * buffer);
             }
         products_done:;
         }
@@ -421,7 +456,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 const Tile x = tile_of(t);
                 // the tile's copies of a block of 64: one box, or the boxes of a run, or of the runs of the slabs
                 int bytes = wide * kRowBytes * kBlocks, wide_boxes = 0, some_boxes = 0, boxes = 0, run = 0, from = 0;  // bytes: of both blocks
-                if (kOp == kDense) columns_of(x, side, from);
+                if (kOne) columns_of(x, side, from);
                 if (runs) {
                     bytes = 0;
                     for (int of = 0; of < kBlocks; ++of) {
@@ -442,8 +477,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     int have = min(per_stage, left);
                     if (side == 0) barrier_expect(full0 + 8 * stage, have * bytes);
                     for (; have > 0; --have, k += kTileInner, at += block_bytes) {
-                        if (kOp == kDense || spread) {
-                            copy_tile_2d<kPair>(at, &p.rows, k, kOp == kDense ? x.first + from : 0, bar);
+                        if (kOne || spread) {
+                            copy_tile_2d<kPair>(at, &p.rows, k, kOne ? x.first + from : 0, bar);
                         } else if (runs) {
                             const int row = s.row[x.group] + x.first + from;
                             if (run >= 64) {
@@ -556,21 +591,47 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             cudaTriggerProgrammaticLaunchCompletion();
         }
         int n = 0;
-        bool met = kOp != kDense || kPair || split == 1;
+        bool met = !kOne || kPair || split == 1;
+        auto sums_read = [&](int buffer) {
+            tcgen05_before_sync();
+            __syncwarp();
+            if (lane == 0) kPair ? barrier_arrive_there(of_first_block(sums_empty0 + 8 * buffer)) : barrier_arrive(sums_empty0 + 8 * buffer);
+        };
         for (int t = tile0; t < tiles; t += tile_step, ++n) {
             const Tile x = tile_of(t);
+            const bool needed = (paired ? quarter * 16 : quarter * 32) < x.height;  // by warp
+            // kDense32: the tile's sum, of those of its parts
+            float total[k32 ? kMaxColumns32 / 32 : 1][16];
+            if constexpr (k32) {
+#pragma unroll
+                for (int g = 0; g < kMaxColumns32 / 32; ++g)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) total[g][j] = 0.0f;
+                bool all = true;
+                for (int chunk = blocks; chunk > sum_blocks && all; chunk -= sum_blocks, ++n) {
+                    all = named_all(1, kFinishers, barrier_wait(sums_full0 + 8 * (n & 1), (n >> 1) & 1, &s.gave_up));
+                    if (!all) break;
+                    tcgen05_after_sync();
+                    add_part(tmem + (n & 1) * kMaxColumns + ((uint32_t)(quarter * 32) << 16), needed, x.columns, half, total);
+                    sums_read(n & 1);
+                }
+                if (!all) break;
+            }
             const int buffer = n & 1;
             bool here = !kGrouped || barrier_wait(list_full0 + 8 * buffer, (n >> 1) & 1, &s.gave_up);
             here = here && barrier_wait(sums_full0 + 8 * buffer, (n >> 1) & 1, &s.gave_up);
             if (!named_all(1, kFinishers, here)) break;  // all warps go on, or none
             tcgen05_after_sync();
             const uint32_t sums = tmem + buffer * kMaxColumns + ((uint32_t)(quarter * 32) << 16);
+            if constexpr (k32) {
+                add_part(sums, needed, x.columns, half, total);
+                sums_read(buffer);
+            }
             // this lane's feature
             const int own = quarter * 32 + lane, within = paired ? own >> 1 : own, f = x.f + within;
             const bool inside = within < x.height && f < p.features, up = paired && (lane & 1);
-            const bool needed = (paired ? quarter * 16 : quarter * 32) < x.height;  // by warp
             float bias = 0.0f;
-            if (kOp == kDense && p.bias != nullptr && inside)
+            if (kOne && p.bias != nullptr && inside)
                 bias = load_any<T>(p.bias, (size_t)(up ? p.features : 0) + f, p.bias_fp32);
             // Finishes columns c0 to c0 + kCount - 1 (an even number). With SwiGLU lanes 2 i and 2 i + 1 hold gate and up of a feature: the
             // first finishes the even columns, the second the odd ones. Values first, then the stores, so that the columns overlap.
@@ -582,8 +643,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     for (int j = 0; j < kCount / 2; ++j) {
                         const int c = c0 + 2 * j + up;
                         add[j] = 0.0f;
-                        if (kOp == kDense && p.residual != nullptr && inside && c < x.columns)
-                            add[j] = load_any<T>(p.residual, (size_t)(x.first + c) * p.residual_stride + f, p.out_fp32);
+                        if (kOne && p.residual != nullptr && inside && c < x.columns)
+                            add[j] = load_any<T>(p.residual, (size_t)(x.first + c) * p.residual_stride + f, k32);
                     }
 #pragma unroll
                     for (int j = 0; j < kCount / 2; ++j) {
@@ -596,8 +657,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     for (int j = 0; j < kCount / 2; ++j) {
                         const int c = c0 + 2 * j + up;
                         if (c >= x.columns) continue;
-                        if (kOp == kDense) {
-                            store_any<T>(p.y, (size_t)(x.first + c) * p.y_stride + f, out[j], p.out_fp32);
+                        if (kOne) {
+                            store_any<T>(p.y, (size_t)(x.first + c) * p.y_stride + f, out[j], k32);
                         } else {
                             // Rounded to the rows' type, since the next product takes 16-bit operands.
                             if (kOp == kLayerUp || s.list[buffer][c] >= 0)
@@ -607,19 +668,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     return;
                 }
                 if (!inside) return;
-                if (kOp == kDense) {
+                if (kOne) {
                     float add[kCount], out[kCount];
 #pragma unroll
                     for (int j = 0; j < kCount; ++j) {
                         add[j] = 0.0f;
                         if (p.residual != nullptr && c0 + j < x.columns)
-                            add[j] = load_any<T>(p.residual, (size_t)(x.first + c0 + j) * p.residual_stride + f, p.out_fp32);
+                            add[j] = load_any<T>(p.residual, (size_t)(x.first + c0 + j) * p.residual_stride + f, k32);
                         out[j] = v[j] + bias;
                     }
                     activate(out, p.activation);
 #pragma unroll
                     for (int j = 0; j < kCount; ++j)
-                        if (c0 + j < x.columns) store_any<T>(p.y, (size_t)(x.first + c0 + j) * p.y_stride + f, out[j] + add[j], p.out_fp32);
+                        if (c0 + j < x.columns) store_any<T>(p.y, (size_t)(x.first + c0 + j) * p.y_stride + f, out[j] + add[j], k32);
                 } else {
 #pragma unroll
                     for (int j = 0; j < kCount; ++j) {
@@ -639,7 +700,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             auto place_of = [&](int c, int within8, int& f0, void*& to, size_t& o) {
                 f0 = x.f + within8;
                 if (within8 >= x.height || f0 >= p.features || c >= x.columns) return 0;
-                if (kOp == kDense) {
+                if (kOne) {
                     o = (size_t)(x.first + c) * p.y_stride + f0;
                     to = p.y;
                     return min(8, p.features - f0);
@@ -661,7 +722,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 int f0;
                 void* to;
                 size_t o;
-                if (kOp != kDense || (p.residual == nullptr && !p.out_fp32)) {
+                if (!kOne || (p.residual == nullptr && !k32)) {
                     const uint4 q = exchange_packed<kStep, T>(v, lane);
                     const int n = place_of(c, within8, f0, to, o);
                     if (n == 8) {
@@ -678,14 +739,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 const int n = place_of(c, within8, f0, to, o);
                 const size_t from = (size_t)(x.first + c) * p.residual_stride + f0;
                 if (n == 8) {
-                    if (p.residual != nullptr) add_eight<T>(v, p.residual, from, p.out_fp32);
-                    put_eight<T>(to, o, v, p.out_fp32);
+                    if (p.residual != nullptr) add_eight<T>(v, p.residual, from, k32);
+                    put_eight<T>(to, o, v, k32);
                 } else if (n > 0) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         if (j >= n) break;
-                        const float add = p.residual != nullptr ? load_any<T>(p.residual, from + j, p.out_fp32) : 0.0f;
-                        store_any<T>(to, o + j, v[j] + add, p.out_fp32);
+                        const float add = p.residual != nullptr ? load_any<T>(p.residual, from + j, k32) : 0.0f;
+                        store_any<T>(to, o + j, v[j] + add, k32);
                     }
                 }
             };
@@ -704,21 +765,22 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 for (int h = 0; h < 2 && !paired; ++h) {
                     float out[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) out[j] = kOp == kDense ? v[8 * h + j] + bias : v[8 * h + j];
-                    if (kOp == kDense) activate(out, p.activation);
+                    for (int j = 0; j < 8; ++j) out[j] = kOne ? v[8 * h + j] + bias : v[8 * h + j];
+                    if (kOne) activate(out, p.activation);
                     store_eight(out, Lanes<1>(), c0 + 8 * h + (lane & 7), quarter * 32 + 8 * (lane >> 3));
                 }
             };
-            if (kOp == kDense && !kPair && split > 1) {
+            if (kOne && !kPair && split > 1) {
                 // The cluster's blocks leave their sums in the ring, which nothing uses any more, and each finishes its share of the
                 // columns, two at a time.
                 float* const left = reinterpret_cast<float*>(ring);
-                for (int c0 = 16 * half; c0 < x.columns && needed; c0 += 32) {
+                for_parts(x.columns, half, total, [&](int c0, float (&part_sums)[16]) {
                     float v[16];
-                    tmem_load_16(sums + c0, v);
+                    if (!needed) return;
+                    if constexpr (!k32) tmem_load_16(sums + c0, v);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) left[(c0 + j) * kTileRows + own] = v[j];
-                }
+                    for (int j = 0; j < 16; ++j) left[(c0 + j) * kTileRows + own] = k32 ? part_sums[j] : v[j];
+                });
                 cluster_sync();
                 met = true;
                 for (int c = 2 * (part + split * half); c < x.columns && needed; c += 4 * split) {
@@ -730,6 +792,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     }
                     finish(c, v);
                 }
+            } else if (k32) {
+                for_parts(x.columns, half, total, [&](int c0, float (&v)[16]) {
+                    if (!needed) return;
+                    if (wide_stores) finish_wide(c0, v);
+                    else finish(c0, v);
+                });
             } else if (needed) {
                 for (int c0 = 16 * half; c0 < x.columns; c0 += 32) {
                     float v[16];
@@ -739,9 +807,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     else finish(c0, v);
                 }
             }
-            tcgen05_before_sync();
-            __syncwarp();
-            if (lane == 0) kPair ? barrier_arrive_there(of_first_block(sums_empty0 + 8 * buffer)) : barrier_arrive(sums_empty0 + 8 * buffer);
+            if constexpr (!k32) sums_read(buffer);
             if (kGrouped) {
                 named_sync(1, kFinishers);
                 if (at == 0) barrier_arrive(list_empty0 + 8 * buffer);
@@ -751,7 +817,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     }
     __syncwarp();
     // What the epilogue's threads meet at, the others meet here: nobody leaves while its sums are read.
-    if (kOp == kDense && !kPair && split > 1) {
+    if (kOne && !kPair && split > 1) {
         if (warp < 4) cluster_sync();
         cluster_sync();
     }

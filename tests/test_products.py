@@ -255,6 +255,17 @@ def test_linear_long_sums(tokens, inputs, outputs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,inputs,outputs", [(600, 7168, 512), (1000, 4096, 2048), (20, 7168, 3000), (5, 7168, 256)])
+def test_linear_sums_of_32_bits_do_not_drift(tokens, inputs, outputs):
+    """The tensor core cuts its sums after every 16 products: up to 2^-23 of what is there, 2/3 of the end's on average. In parts of at most 896, 56 of them,
+    that is 56 * 2/3 * 2^-23 in the 2-norm even if all go one way; 7168 at once were 8e-6 off."""
+    g = generator(tokens, inputs, 32)
+    x, w = normal(g, tokens, inputs, dtype=torch.bfloat16).to(DEV), normal(g, outputs, inputs, std=inputs ** -0.5, dtype=torch.bfloat16).to(DEV)
+    want = x.double() @ w.double().t()
+    assert float((linear(x, w, out_dtype=torch.float32).double() - want).norm() / want.norm()) < 56 * 2 / 3 * 2.0 ** -23
+
+
+@pytest.mark.gpu
 def test_linear_strides_shapes_and_views():
     g = generator(5)
     base = normal(g, 80, 400, dtype=torch.bfloat16).to(DEV)
