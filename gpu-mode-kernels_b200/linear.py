@@ -64,9 +64,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     out_dtype = out_dtype or x.dtype
     if out_dtype not in (x.dtype, torch.float32):
         refuse(f"out_dtype must be {x.dtype} or torch.float32, got {out_dtype}")
-    if weight.stride(1) != 1 or weight.stride(0) < inputs or weight.stride(0) % 8 or weight.data_ptr() % 16:
+    if weight.stride(1) != 1 or (rows > 1 and (weight.stride(0) < inputs or weight.stride(0) % 8)) or weight.data_ptr() % 16:
         refuse("weight must have contiguous rows, 16-byte aligned")
-    if bias is not None and (bias.dtype not in (x.dtype, torch.float32) or tuple(bias.shape) != (rows,) or bias.stride(0) != 1
+    if bias is not None and (bias.dtype not in (x.dtype, torch.float32) or tuple(bias.shape) != (rows,) or not bias.is_contiguous()
                              or bias.get_device() != device):
         refuse(f"bias must be a contiguous [{rows}] of {x.dtype} or torch.float32 on {x.device}, got {tuple(bias.shape)} {bias.dtype}")
     shape = (*x.shape[:-1], outputs)

@@ -283,6 +283,8 @@ def test_linear_strides_shapes_and_views():
     check_linear(base.view(4, 20, 400)[:, :, :64], w[:, :64])
     check_linear(base[0, :64], w[:, :64], residual=base[1, :96])
     check_linear(base[:1, :64], w[:1, :64])
+    odd = normal(g, 3, 403, dtype=torch.bfloat16).to(DEV)
+    check_linear(base[:5, :64], torch.as_strided(w, (1, 64), (7, 1)), odd[:, 0][:1])  # strides of a length of one say nothing
     assert linear(base[:0, :64], w[:, :64]).shape == (0, 96)
     assert linear(base.view(4, 20, 400)[:, :0, :64], w[:, :64]).shape == (4, 0, 96)
 
