@@ -184,6 +184,21 @@ def test_gate_rows_with_nothing_to_choose():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_gate_excluded_experts_stay_out_whatever_their_bias(score):
+    logits, bias = torch.full((4, 70), -float("inf")), torch.zeros(70)
+    logits[:, 40:45] = torch.arange(5.0)
+    logits[1, 66] = -1e30         # small, but a number
+    logits[2, 41:45] = -float("inf")  # one left, three asked for
+    logits[3] = -float("inf")
+    bias[:8], bias[66] = 5.0, 2.0
+    idx, w = topk_gate(logits.to(DEV), 3, score=score, bias=bias.to(DEV), renormalize=False)
+    assert idx.tolist() == [[44, 43, 42], [66, 44, 43], [40, 0, 1], [0, 1, 2]]
+    s = torch.softmax(logits.double(), 1).nan_to_num() if score == "softmax" else torch.sigmoid(logits.double())
+    torch.testing.assert_close(w.cpu().double(), s.gather(1, idx.cpu().long()), rtol=2.0 ** -18, atol=1e-38)
+
+
+@pytest.mark.gpu
 def test_gate_refusals():
     l = torch.zeros(4, 16, device=DEV)
     for call in (lambda: topk_gate(l.double(), 2), lambda: topk_gate(l[0], 2), lambda: topk_gate(l, 0), lambda: topk_gate(l, 17),
