@@ -536,17 +536,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                         for (int c = lane; c < x.columns; c += 32) s.scale[buffer][c] = p.weights_of[s.list[buffer][c]];
                     }
                 } else {
-                    // the row of the slabs that stands at a column, and whether it is a valid one
+                    // The row of the slabs that stands at a column, and whether it is a valid one. The sources' counts are read once for all
+                    // columns (one after the other for each column they took longer than a tile's products).
+                    int have[A2A_MAX_WORLD];
+#pragma unroll
+                    for (int src = 0; src < A2A_MAX_WORLD; ++src) have[src] = src < p.world ? slab_rows(x.group, src) : 0;
                     auto row_at = [&](int c, bool& valid) {
-                        int r = x.first + c, src = 0, have = 0;
-                        for (; src < p.world - 1; ++src) {
-                            have = slab_rows(x.group, src);
-                            const int room = (have + slab_step - 1) & -slab_step;
-                            if (r < room) break;
-                            r -= room;
+                        int r = x.first + c, src = 0, rows = 0;
+#pragma unroll
+                        for (int i = 0, begin = 0; i < A2A_MAX_WORLD; ++i) {
+                            if (i < p.world && x.first + c >= begin) src = i, r = x.first + c - begin, rows = have[i];
+                            begin += (have[i] + slab_step - 1) & -slab_step;
                         }
-                        if (src == p.world - 1) have = slab_rows(x.group, src);
-                        valid = r < have;
+                        valid = r < rows;
                         return (x.group * p.world + src) * p.capacity + r;
                     };
                     bool valid;
@@ -803,11 +805,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     float v[16];
                     if (spread) tmem_load_spread(sums, [&](int j) { return s.list[buffer][min(c0 + j, x.columns - 1)] / p.topk; }, v);
                     else tmem_load_16(sums + c0, v);
+                    if (c0 + 32 >= x.columns) sums_read(buffer);
                     if (wide_stores) finish_wide(c0, v);
                     else finish(c0, v);
                 }
             }
-            if constexpr (!k32) sums_read(buffer);
+            if (!k32 && (!needed || 16 * half >= x.columns)) sums_read(buffer);  // this warp had none to read
             if (kGrouped) {
                 named_sync(1, kFinishers);
                 if (at == 0) barrier_arrive(list_empty0 + 8 * buffer);
