@@ -298,6 +298,34 @@ __device__ __forceinline__ void tmem_load_16(uint32_t tmem, float (&v)[16]) {
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// The same as matrix fragments: v[8 h + 4 c + 2 r + j] is of lane 16 h + 8 r + (own lane) / 4 and column 8 c + 2 (own lane % 4) + j.
+__device__ __forceinline__ void tmem_load_fragments(uint32_t tmem, float (&v)[16]) {
+    uint32_t r[16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[8 * h]), "=r"(r[8 * h + 1]), "=r"(r[8 * h + 2]), "=r"(r[8 * h + 3]), "=r"(r[8 * h + 4]), "=r"(r[8 * h + 5]),
+                       "=r"(r[8 * h + 6]), "=r"(r[8 * h + 7])
+                     : "r"(tmem + ((uint32_t)(16 * h) << 16)));
+    // the values go through the wait, so that nothing reads them ahead of it
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Two values in 16 bits each, the first one lower.
+template <typename T>
+__device__ __forceinline__ uint32_t packed(float low, float high) {
+    alignas(4) const T two[2] = {Element<T>::from_float(low), Element<T>::from_float(high)};
+    return *reinterpret_cast<const uint32_t*>(two);
+}
+// Four matrices of 8 by 8 fragments of 16 bits, turned over on their way into shared memory; lane i has the place of row i % 8 of matrix i / 8.
+__device__ __forceinline__ void store_turned(uint32_t to, const uint32_t (&q)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared::cta.b16 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                 : "memory");
+}
+
 // 16 columns that need not be neighbours: of() gives each one's, the same in all lanes.
 template <typename Of>
 __device__ __forceinline__ void tmem_load_spread(uint32_t tmem, Of of, float (&v)[16]) {

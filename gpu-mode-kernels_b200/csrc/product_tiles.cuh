@@ -146,7 +146,10 @@ struct TilesShared {
     int2 box[2][kMaxColumns / 8];  // kSlab*: boxes of 64, of 32 and of 8 rows: first row and column
     int boxes[2][3];               // where each kind ends
     int box_rows[2];               // rows of all boxes, of both blocks of a pair
-    short expert[kCached];         // kLayer*: expert of a pair, -1 for none
+    union {
+        short expert[kCached];                                 // kLayer*: expert of a pair, -1 for none
+        alignas(16) uint16_t turned[kFinishers / 32][16][32];  // others: columns by features of a warp of the epilogue, on their way out
+    };
 };
 // An operand of less than 128 rows at the end of the ring is read beyond it.
 static_assert(sizeof(TilesShared) >= kTileRows * kRowBytes, "operands of 128 rows end within the shared memory");
@@ -717,6 +720,57 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 to = p.y;
                 return row >= 0 ? 8 : 0;
             };
+            // A column's features `q` to their places.
+            auto store_packed = [&](const uint4& q, int c, int within8) {
+                int f0;
+                void* to;
+                size_t o;
+                const int n = place_of(c, within8, f0, to, o);
+                if (n == 8) {
+                    *reinterpret_cast<uint4*>(static_cast<T*>(to) + o) = q;
+                } else if (n > 0) {  // the last ones
+                    const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < n) reinterpret_cast<uint16_t*>(to)[o + j] = (uint16_t)(word[j / 2] >> 16 * (j & 1));
+                }
+            };
+            // Without SwiGLU, residual and 32-bit results the exchange is the shared memory's: fragments of the sums go there turned over, and come back
+            // as 8 features of a column. (16384 rows of 1024 to 2048: 51 us, with shuffles 60; 8192 of 512 to 4096 35 and 55.)
+            const bool turns = kOp != kLayerDown && !k32 && !kUp && wide_stores && !paired && (!kOne || p.residual == nullptr);
+            float biases[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (kOne && turns && p.bias != nullptr)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at_row = quarter * 32 + 8 * j + (lane >> 2);
+                    if (at_row < x.height && x.f + at_row < p.features) biases[j] = load_any<T>(p.bias, (size_t)x.f + at_row, p.bias_fp32);
+                }
+            auto finish_turned = [&](int c0, float (&v)[16]) {
+                if (kOne) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] += biases[2 * (i >> 3) + (i >> 1 & 1)];
+                    activate(v, p.activation);
+                }
+                const uint32_t mine = shared_addr(s.turned[warp - 4]);
+                // (16 bytes of neighbouring rows lie apart, so that the eight of a matrix come from all banks)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t q[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) q[j] = packed<T>(v[8 * (j >> 1) + 4 * c + 2 * (j & 1)], v[8 * (j >> 1) + 4 * c + 2 * (j & 1) + 1]);
+                    store_turned(mine + (8 * c + (lane & 7)) * 64 + (((lane >> 3) ^ (lane >> 1 & 3)) << 4), q);
+                }
+                __syncwarp();
+                uint4 q[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c = 8 * h + (lane >> 2);
+                    q[h] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(s.turned[warp - 4]) + c * 64 + (((lane & 3) ^ (c >> 1 & 3)) << 4));
+                }
+                __syncwarp();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) store_packed(q[h], c0 + 8 * h + (lane >> 2), quarter * 32 + 8 * (lane & 3));
+            };
             // kStep: what the columns of the eight values differ by in lanes. Inner values are rounded to the rows' type, since the next product
             // takes 16-bit operands.
             auto store_eight = [&](float (&v)[8], auto step, int c, int within8) {
@@ -725,16 +779,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 void* to;
                 size_t o;
                 if (!kOne || (p.residual == nullptr && !k32)) {
-                    const uint4 q = exchange_packed<kStep, T>(v, lane);
-                    const int n = place_of(c, within8, f0, to, o);
-                    if (n == 8) {
-                        *reinterpret_cast<uint4*>(static_cast<T*>(to) + o) = q;
-                    } else if (n > 0) {  // the last ones
-                        const uint32_t word[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (j < n) reinterpret_cast<uint16_t*>(to)[o + j] = (uint16_t)(word[j / 2] >> 16 * (j & 1));
-                    }
+                    store_packed(exchange_packed<kStep, T>(v, lane), c, within8);
                     return;
                 }
                 exchange_eight<kStep>(v, lane);
@@ -804,9 +849,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 for (int c0 = 16 * half; c0 < x.columns; c0 += 32) {
                     float v[16];
                     if (spread) tmem_load_spread(sums, [&](int j) { return s.list[buffer][min(c0 + j, x.columns - 1)] / p.topk; }, v);
+                    else if (turns) tmem_load_fragments(sums + c0, v);
                     else tmem_load_16(sums + c0, v);
                     if (c0 + 32 >= x.columns) sums_read(buffer);
-                    if (wide_stores) finish_wide(c0, v);
+                    if (turns) finish_turned(c0, v);
+                    else if (wide_stores) finish_wide(c0, v);
                     else finish(c0, v);
                 }
             }
