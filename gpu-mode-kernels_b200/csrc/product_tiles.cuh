@@ -52,6 +52,7 @@ constexpr int kTmemColumns = 512;
 constexpr int kSpreadTokens = 64;  // 40 to 100 tokens take the same either way
 constexpr int kPieceRows = 32;  // operand rows of a box of a tile that is less than full
 constexpr int kMaxSplit = 8;
+constexpr int kTilesAhead = 64;
 // The tensor core cuts the sums it adds to: a sum of 7168 products came out 8e-6 off, of the 2-norm, where fp32 additions are 9e-7 off. For a result
 // of 32 bits a sum in tensor memory therefore is of about 512 of the inner length (5e-7 off), and the epilogue's threads add the parts up in
 // registers, which hold 128 columns. A sum of up to 896 is left whole (9e-7; 256 outputs of 7168, 16 rows, 6.5 us in parts and 5.9 at once), but for
@@ -129,6 +130,10 @@ __host__ __device__ __forceinline__ Rounds rounds_of(int tiles, int blocks, int 
 }
 
 
+struct Tile {
+    int group, f, height, first, columns;  // matrix, first feature, features, first column, columns
+};
+
 struct TilesShared {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t sums_full[2], sums_empty[2];
@@ -145,6 +150,7 @@ struct TilesShared {
     float scale[2][kMaxColumns];
     int2 box[2][kMaxColumns / 8];  // kSlab*: boxes of 64, of 32 and of 8 rows: first row and column
     int boxes[2][3];               // where each kind ends
+    Tile tile[kTilesAhead];        // the block's first ones
     int box_rows[2];               // rows of all boxes, of both blocks of a pair
     union {
         short expert[kCached];                                 // kLayer*: expert of a pair, -1 for none
@@ -179,9 +185,6 @@ __device__ __forceinline__ void add_part(uint32_t sums, bool needed, int columns
     });
 }
 
-struct Tile {
-    int group, f, height, first, columns;  // matrix, first feature, features, first column, columns
-};
 
 
 __host__ __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
@@ -235,7 +238,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     auto slab_rows = [&](int g, int src) { return min(max(p.counts[(size_t)src * 4 * p.groups + g], 0), p.capacity); };
     auto slab_columns = [&](int g, int step) {
         int n = 0;
-        for (int src = 0; src < p.world; ++src) n += (slab_rows(g, src) + step - 1) & -step;
+#pragma unroll
+        for (int src = 0; src < A2A_MAX_WORLD; ++src)
+            if (src < p.world) n += (slab_rows(g, src) + step - 1) & -step;
         return n;
     };
 
@@ -358,6 +363,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         x.columns = min(columns, count - x.first);
         return x;
     };
+    // Over experts the roles find their tiles in a table, the first ones at least: working one out takes 900 cycles, in which the ring empties.
+    if (kGrouped) {
+        if (tid < kTilesAhead && tile0 + tid * tile_step < tiles) s.tile[tid] = tile_of(tile0 + tid * tile_step);
+        __syncthreads();
+    }
+    auto tile_at = [&](int n) { return kGrouped && n < kTilesAhead ? s.tile[n] : tile_of(tile0 + n * tile_step); };
     // columns of a tile's product, and of those the ones that block `of` of the pair copies
     auto product_columns = [&](const Tile& x) {
         if (kOne && kPair) return columns;
@@ -386,8 +397,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         if (elect_one()) {
             int stage = 0;
             uint32_t phase = 1;
-            for (int t = tile0; t < tiles; t += tile_step) {
-                const Tile x = tile_of(t);
+            for (int t = tile0, i = 0; t < tiles; t += tile_step, ++i) {
+                const Tile x = tile_at(i);
                 const int f = x.f, h1 = x.height;
                 const bool whole = !kGrouped || h1 == p.full;  // a box of all features, or pieces
                 const int bytes = whole ? (paired ? 2 : 1) * h1 * kRowBytes : parts_of(h1, piece) * kPieceRows * kRowBytes;
@@ -418,8 +429,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             int stage = 0, n = 0;
             uint32_t phase = 0;
             const uint64_t ring_descriptor = operand_descriptor(ring0);
-            for (int t = tile0; t < tiles; t += tile_step) {
-                const Tile x = tile_of(t);
+            for (int t = tile0, i = 0; t < tiles; t += tile_step, ++i) {
+                const Tile x = tile_at(i);
                 const uint32_t descriptor = instruction_descriptor(Element<T>::kFormat, kTileRows * kBlocks, product_columns(x));
                 for (int chunk = blocks; chunk > 0; ++n) {
                     // a sum in tensor memory: the whole inner length, or for a result of 32 bits a part of it
@@ -455,8 +466,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         if (elect_one()) {
             int stage = 0, n = 0;
             uint32_t phase = 1;
-            for (int t = tile0; t < tiles; t += tile_step, ++n) {
-                const Tile x = tile_of(t);
+            for (int t = tile0, i = 0; t < tiles; t += tile_step, ++n, ++i) {
+                const Tile x = tile_at(i);
                 // the tile's copies of a block of 64: one box, or the boxes of a run, or of the runs of the slabs
                 int bytes = wide * kRowBytes * kBlocks, wide_boxes = 0, some_boxes = 0, boxes = 0, run = 0, from = 0;  // bytes: of both blocks
                 if (kOne) columns_of(x, side, from);
@@ -508,8 +519,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     } else if (warp == 3) {
         if (kGrouped) {
             int n = 0;
-            for (int t = tile0; t < tiles; t += tile_step, ++n) {
-                const Tile x = tile_of(t);
+            for (int t = tile0, i = 0; t < tiles; t += tile_step, ++n, ++i) {
+                const Tile x = tile_at(i);
                 const int buffer = n & 1;
                 if (!__all_sync(0xffffffffu, barrier_wait(list_empty0 + 8 * buffer, ((n >> 1) & 1) ^ 1, &s.gave_up))) break;
                 if (kLayer) {
@@ -602,8 +613,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             __syncwarp();
             if (lane == 0) kPair ? barrier_arrive_there(of_first_block(sums_empty0 + 8 * buffer)) : barrier_arrive(sums_empty0 + 8 * buffer);
         };
-        for (int t = tile0; t < tiles; t += tile_step, ++n) {
-            const Tile x = tile_of(t);
+        for (int t = tile0, i = 0; t < tiles; t += tile_step, ++n, ++i) {
+            const Tile x = tile_at(i);
             const bool needed = (paired ? quarter * 16 : quarter * 32) < x.height;  // by warp
             // kDense32: the tile's sum, of those of its parts
             float total[k32 ? kMaxColumns32 / 32 : 1][16];
