@@ -73,21 +73,21 @@ int sm_count(int* sms) {
 }
 
 // Lets the kernel have its shared memory on the current device.
-template <TilesOp kOp, typename T, bool kPair>
+template <TilesOp kOp, typename T, Together kTogether>
 int opt_in() {
     static std::atomic<unsigned long long> opted{0};  // a bit a device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return -(int)e;
     if (dev < 64 && (opted.load(std::memory_order_acquire) >> dev & 1)) return A2A_OK;
-    e = cudaFuncSetAttribute((const void*)&product_tiles_kernel<kOp, T, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTilesSharedBytes);
+    e = cudaFuncSetAttribute((const void*)&product_tiles_kernel<kOp, T, kTogether>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTilesSharedBytes);
     if (e != cudaSuccess) return -(int)e;
     if (dev < 64) opted.fetch_or(1ull << dev, std::memory_order_release);
     return A2A_OK;
 }
 
 // How many clusters of `size` blocks run at once: they do not come to lie on every SM.
-template <TilesOp kOp, typename T, bool kPair>
+template <TilesOp kOp, typename T, Together kTogether>
 int most_clusters(int size) {
     static std::atomic<int> known[kMaxSplit + 1];  // one more than the number; of the first device that asked, as all are alike
     int n = known[size].load(std::memory_order_relaxed);
@@ -102,8 +102,8 @@ int most_clusters(int size) {
         config.dynamicSmemBytes = kTilesSharedBytes;
         config.attrs = &attr;
         config.numAttrs = 1;
-        if (opt_in<kOp, T, kPair>() != A2A_OK ||
-            cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T, kPair>), &config) != cudaSuccess) {
+        if (opt_in<kOp, T, kTogether>() != A2A_OK ||
+            cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T, kTogether>), &config) != cudaSuccess) {
             cudaGetLastError();
             return 0;
         }
@@ -132,11 +132,11 @@ int launch(const void* fn, dim3 grid, int threads, size_t shared, int cluster, v
     return e == cudaSuccess ? A2A_OK : -(int)e;
 }
 
-template <TilesOp kOp, typename T, bool kPair = false>
+template <TilesOp kOp, typename T, Together kTogether = kAlone>
 int launch_tiles(const TilesParams& p, int grid, int cluster, cudaStream_t st) {
-    const int rc = opt_in<kOp, T, kPair>();
+    const int rc = opt_in<kOp, T, kTogether>();
     if (rc != A2A_OK) return rc;
-    return launch(reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T, kPair>), grid, kTilesThreads, kTilesSharedBytes, cluster, const_cast<TilesParams*>(&p), st);
+    return launch(reinterpret_cast<const void*>(&product_tiles_kernel<kOp, T, kTogether>), grid, kTilesThreads, kTilesSharedBytes, cluster, const_cast<TilesParams*>(&p), st);
 }
 
 // How a dense product is cut: features and columns of a tile, blocks that share a tile's inner length, or pairs of blocks.
@@ -165,7 +165,7 @@ DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
             int height = parts_of(a.outputs, down);
             if (columns > 16 && most % 8 == 0) height = (height + 7) & ~7;  // stores of sixteen bytes
             const int tiles = parts_of(a.outputs, height) * across;
-            if (split > 1 && tiles > most_clusters<kOp, T, false>(split)) return;
+            if (split > 1 && tiles > most_clusters<kOp, T, kCuts>(split)) return;
             const int busy = std::min(tiles * split, sms), rounds = split > 1 ? 1 : parts_of(tiles, sms);
             const float block = block_ns(paired ? 2 * height : height, columns, columns, busy / (6500.0f * across));
             const float t = rounds * parts_of(blocks, split) * std::max(block, 1.3f * std::min(parts_of(a.outputs, height), sms)) + tail +
@@ -178,13 +178,13 @@ DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
             if (down > least_down && parts_of(a.outputs, down) >= std::min(most, 8)) consider(down, 1);
         }
         for (int split = 2; split <= std::min(kMaxSplit, blocks); ++split) {
-            const int room = most_clusters<kOp, T, false>(split), down = room / across;
+            const int room = most_clusters<kOp, T, kCuts>(split), down = room / across;
             if (down < least_down) break;
             consider(least_down, split);
             if (down > least_down && parts_of(a.outputs, down) >= std::min(most, 8)) consider(down, split);
         }
         if (width % 32 == 0) {
-            const int wide = (parts_of(a.tokens, across) + 31) / 32 * 32, tiles = parts_of(a.outputs, 2 * most) * across, units = most_clusters<kOp, T, true>(2);
+            const int wide = (parts_of(a.tokens, across) + 31) / 32 * 32, tiles = parts_of(a.outputs, 2 * most) * across, units = most_clusters<kOp, T, kPairs>(2);
             if (units < 1) continue;
             const float t = parts_of(tiles, units) * blocks * block_ns(paired ? 2 * most : most, wide, wide / 2, 2 * std::min(tiles, units) / (6500.0f * across)) + tail;
             if (t < least * 0.999f) least = t, best = DensePlan{most, wide, 1, true};
@@ -210,10 +210,10 @@ int linear_of(const a2a_linear_args& a, int sms, cudaStream_t st) {
     if (rc != A2A_OK) return rc;
     if (plan.pair) {
         const int tiles = parts_of(a.outputs, 2 * plan.height) * parts_of(a.tokens, plan.columns);
-        return launch_tiles<kOp, T, true>(p, 2 * std::min(tiles, most_clusters<kOp, T, true>(2)), 2, st);
+        return launch_tiles<kOp, T, kPairs>(p, 2 * std::min(tiles, most_clusters<kOp, T, kPairs>(2)), 2, st);
     }
     const int tiles = parts_of(a.outputs, plan.height) * parts_of(a.tokens, plan.columns);
-    return launch_tiles<kOp, T>(p, plan.split > 1 ? tiles * plan.split : std::min(tiles, sms), plan.split, st);
+    return plan.split > 1 ? launch_tiles<kOp, T, kCuts>(p, tiles * plan.split, plan.split, st) : launch_tiles<kOp, T>(p, std::min(tiles, sms), 1, st);
 }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -288,12 +288,12 @@ int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {
     p.columns = kMaxColumns;
     int rc = expert_maps(p, a.dtype, a.gate_up, a.local_experts, a.inner, true, a.hidden_dim);
     if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.rows, rows);
-    if (rc == A2A_OK) rc = launch_tiles<kSlabUp, T, true>(p, 2 * std::max(1, most_clusters<kSlabUp, T, true>(2)), 2, st);
+    if (rc == A2A_OK) rc = launch_tiles<kSlabUp, T, kPairs>(p, 2 * std::max(1, most_clusters<kSlabUp, T, kPairs>(2)), 2, st);
     if (rc != A2A_OK) return rc;
     p.y = a.out, p.wide_stores = aligned(a.out);
     rc = expert_maps(p, a.dtype, a.down, a.local_experts, a.hidden_dim, false, a.inner);
     if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.workspace, inner_rows(a.local_experts, a.world, a.capacity));
-    return rc == A2A_OK ? launch_tiles<kSlabDown, T, true>(p, 2 * std::max(1, most_clusters<kSlabDown, T, true>(2)), 2, st) : rc;
+    return rc == A2A_OK ? launch_tiles<kSlabDown, T, kPairs>(p, 2 * std::max(1, most_clusters<kSlabDown, T, kPairs>(2)), 2, st) : rc;
 }
 
 bool dtype16(int dtype) { return dtype == A2A_DTYPE_BF16 || dtype == A2A_DTYPE_FP16; }

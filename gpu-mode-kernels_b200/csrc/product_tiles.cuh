@@ -39,6 +39,9 @@ namespace {
 
 // kDense32: with a result of 32 bits
 enum TilesOp { kDense, kDense32, kLayerUp, kLayerDown, kSlabUp, kSlabDown };
+// Blocks have tiles of their own; are pairs, which share tiles; or clusters, whose blocks have a part of a tile's inner length each. (A kernel for each:
+// the instructions of a short one come from far away, and those of the others between them cost a small product 0.3 us.)
+enum Together { kAlone, kPairs, kCuts };
 
 constexpr int kTileRows = 128, kTileInner = 64, kMaxColumns = 256;
 constexpr int kRowBytes = kTileInner * 2;
@@ -196,8 +199,9 @@ __host__ __device__ __forceinline__ float block_ns(int rows, int columns, int he
     return fmaxf(fmaxf(fmaxf(memory, cache), products), 110.0f) + 10.0f;
 }
 
-template <TilesOp kOp, typename T, bool kPair>
+template <TilesOp kOp, typename T, Together kTogether>
 __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const __grid_constant__ TilesParams p) {
+    constexpr bool kPair = kTogether == kPairs, kCut = kTogether == kCuts;
     constexpr bool k32 = kOp == kDense32, kOne = kOp == kDense || k32, kGrouped = !kOne, kLayer = kOp == kLayerUp || kOp == kLayerDown, kSlab = kOp == kSlabUp || kOp == kSlabDown;
     constexpr bool kUp = kOp == kLayerUp || kOp == kSlabUp;
     const bool first = kOne || (kOp == kLayerUp && !p.sorted) || kOp == kSlabUp;  // nothing of the same call runs before it
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     const int per_stage = min(blocks_all, max(1, quotient(kStageBytes + block_bytes / 2, block_bytes)));
     const int stages = min(kMaxStages, quotient(kRingBytes, block_bytes * per_stage));
     // this block's part of the inner length, and its tiles
-    const int split = kOne && !kPair ? p.split : 1, part = kOne && !kPair ? (int)blockIdx.x % split : 0;
+    const int split = kCut ? p.split : 1, part = kCut ? (int)blockIdx.x % split : 0;
     const int block0 = blocks_all * part / split, blocks = blocks_all * (part + 1) / split - block0;
     const int tile0 = (int)blockIdx.x / (kBlocks * split), tile_step = units / split;
 
@@ -607,7 +611,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             cudaTriggerProgrammaticLaunchCompletion();
         }
         int n = 0;
-        bool met = !kOne || kPair || split == 1;
+        bool met = !kCut;
         auto sums_read = [&](int buffer) {
             tcgen05_before_sync();
             __syncwarp();
@@ -828,7 +832,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     store_eight(out, Lanes<1>(), c0 + 8 * h + (lane & 7), quarter * 32 + 8 * (lane >> 3));
                 }
             };
-            if (kOne && !kPair && split > 1) {
+            if (kCut) {
                 // The cluster's blocks leave their sums in the ring, which nothing uses any more, and each finishes its share of the
                 // columns, two at a time.
                 float* const left = reinterpret_cast<float*>(ring);
@@ -878,7 +882,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     }
     __syncwarp();
     // What the epilogue's threads meet at, the others meet here: nobody leaves while its sums are read.
-    if (kOne && !kPair && split > 1) {
+    if (kCut) {
         if (warp < 4) cluster_sync();
         cluster_sync();
     }
