@@ -256,7 +256,6 @@ int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
     TilesParams p{};
     p.groups = a.experts, p.tokens = a.tokens, p.topk = a.topk, p.indices = a.topk_idx, p.weights_of = a.topk_weights;
     p.hidden = space, p.parts = reinterpret_cast<float*>(space + at.parts);
-    p.wide_stores = 1;
     p.columns = kMaxColumns;
     int rc = expert_maps(p, a.dtype, a.gate_up, a.experts, a.inner, true, a.hidden_dim);
     p.sorted = a.tokens > kSpreadTokens;
@@ -284,7 +283,7 @@ template <typename T>
 int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {
     const long long rows = (long long)a.local_experts * a.world * a.capacity;
     TilesParams p{};
-    p.groups = a.local_experts, p.counts = a.counts, p.world = a.world, p.capacity = a.capacity, p.hidden = a.workspace, p.wide_stores = 1;
+    p.groups = a.local_experts, p.counts = a.counts, p.world = a.world, p.capacity = a.capacity, p.hidden = a.workspace;
     p.columns = kMaxColumns;
     int rc = expert_maps(p, a.dtype, a.gate_up, a.local_experts, a.inner, true, a.hidden_dim);
     if (rc == A2A_OK) rc = run_maps(p, a.dtype, a.rows, rows);

@@ -79,7 +79,7 @@ struct TilesParams {
     int tokens;
     // kDense: the epilogue
     int activation, bias_fp32;
-    int wide_stores;  // rows of y, and of the residual, begin on 16 bytes
+    int wide_stores;  // rows of y, and of the residual, begin on 16 bytes; of kSlabDown too
     const void* bias;
     const void* residual;
     long long residual_stride;
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     for (int j = 0; j < kCount / 2; ++j) {
                         const int c = c0 + 2 * j + up;
                         add[j] = 0.0f;
-                        if (kOne && p.residual != nullptr && inside && c < x.columns)
+                        if (p.residual != nullptr && inside && c < x.columns)
                             add[j] = load_any<T>(p.residual, (size_t)(x.first + c) * p.residual_stride + f, k32);
                     }
 #pragma unroll
@@ -677,13 +677,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     for (int j = 0; j < kCount / 2; ++j) {
                         const int c = c0 + 2 * j + up;
                         if (c >= x.columns) continue;
-                        if (kOne) {
-                            store_any<T>(p.y, (size_t)(x.first + c) * p.y_stride + f, out[j], k32);
-                        } else {
-                            // Rounded to the rows' type, since the next product takes 16-bit operands.
-                            if (kOp == kLayerUp || s.list[buffer][c] >= 0)
-                                static_cast<T*>(p.hidden)[(size_t)(s.row[x.group] + x.first + c) * p.features + f] = Element<T>::from_float(out[j]);
-                        }
+                        store_any<T>(p.y, (size_t)(x.first + c) * p.y_stride + f, out[j], k32);
                     }
                     return;
                 }
@@ -715,7 +709,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
             // The same for whole 16 columns and features in eights, with 16-byte stores: three exchanges between lanes turn a lane's 8 columns of a
             // feature into 8 features of a column. (A store of two bytes for each value: 132 us for experts on slabs of 7000 rows of 2048
             // where this takes 117.)
-            const bool wide_stores = kOp != kLayerDown && p.wide_stores && (x.f & 7) == 0 && (x.height & 7) == 0;
+            // (inner values: always)
+            const bool wide_stores = kUp || (kOp != kLayerDown && p.wide_stores && (x.f & 7) == 0 && (x.height & 7) == 0);
             // where features f0 to f0 + 7 of column c go, and how many of them there are; none: 0
             auto place_of = [&](int c, int within8, int& f0, void*& to, size_t& o) {
                 f0 = x.f + within8;
@@ -869,7 +864,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     if (c0 + 32 >= x.columns) sums_read(buffer);
                     if (turns) finish_turned(c0, v);
                     else if (wide_stores) finish_wide(c0, v);
-                    else finish(c0, v);
+                    else if constexpr (!kUp) finish(c0, v);
                 }
             }
             if (!k32 && (!needed || 16 * half >= x.columns)) sums_read(buffer);  // this warp had none to read
