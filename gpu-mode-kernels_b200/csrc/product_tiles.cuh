@@ -231,6 +231,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     if (warp == 1) tmem_alloc<kPair>(&s.tmem, kTmemColumns);
     if (warp == 2 && lane < (!kGrouped ? 2 : kOp == kLayerUp && !p.sorted ? 3 : 4))
         prefetch_map(lane == 0 ? &p.weights : lane == 1 ? &p.rows : lane == 2 ? &p.weights_piece : &p.rows_few);
+    if (kLayer)
+#pragma unroll 1
+        for (int g = tid; g < p.groups; g += kTilesThreads) s.count[g] = 0;
     // A call's later launches read weights, indices and counts ahead of this: what wrote those was through before the call's first launch let
     // the second one begin.
     if (first) {
@@ -250,43 +253,63 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
 
     // ---- how many columns every group has, and so the tiles ----
     int columns = p.columns, height = p.full, slab_step = 8;
-    if (kGrouped) {
-        for (int g = tid; g < p.groups; g += kTilesThreads) s.count[g] = kSlab ? slab_columns(g, 8) : 0;
+    if (kLayer) {
+        const int pairs = p.tokens * p.topk;
+        int next = tid < pairs ? p.indices[tid] : -1;  // on its way while the threads meet
         __syncthreads();
-        if (kLayer) {
-            for (int i = tid; i < p.tokens * p.topk; i += kTilesThreads) {
-                int e = p.indices[i];
-                if (e < 0 || e >= p.groups) e = -1;
-                if (i < kCached) s.expert[i] = (short)e;
-                if (e >= 0) atomicAdd(&s.count[e], 1);
-            }
-            __syncthreads();
+#pragma unroll 1
+        for (int i = tid; i < pairs; i += kTilesThreads) {
+            const int e = next < 0 || next >= p.groups ? -1 : next;
+            if (i + kTilesThreads < pairs) next = p.indices[i + kTilesThreads];
+            if (i < kCached) s.expert[i] = (short)e;
+            if (e >= 0) atomicAdd(&s.count[e], 1);
         }
+        __syncthreads();
+    }
+    if (kSlab) {
         int most = 0;
-        for (int g = tid; g < p.groups; g += kTilesThreads) most = max(most, s.count[g]);
+#pragma unroll 1
+        for (int g = tid; g < p.groups; g += kTilesThreads) most = max(most, s.count[g] = slab_columns(g, 8));
         most = __reduce_max_sync(0xffffffffu, most);
+        __syncthreads();  // `largest` is 0
         if (lane == 0) atomicMax(&s.largest, most);
         __syncthreads();
-        if (kSlab && s.largest > kMaxColumns) {
+        if (s.largest > kMaxColumns) {
             // more than a tile of columns: columns without a row cost less than boxes of eight
             slab_step = kManyStep;
+#pragma unroll 1
             for (int g = tid; g < p.groups; g += kTilesThreads) s.count[g] = slab_columns(g, slab_step);
             __syncthreads();
         }
-        columns = min(p.columns, (max(s.largest, 1) + kColumnStep - 1) / kColumnStep * kColumnStep);
+    }
+    auto widest = [&](int largest) { return min(p.columns, (max(largest, 1) + kColumnStep - 1) / kColumnStep * kColumnStep); };
+    if (kGrouped) {
         if (warp == 0) {
-            int run = 0, rows = 0;
-            for (int g0 = 0; g0 < p.groups; g0 += 32) {
-                const int g = g0 + lane, n = g < p.groups ? s.count[g] : 0;
-                const int own = parts_of(n, columns);
-                int sum = own, sum_rows = n;
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int left = __shfl_up_sync(0xffffffffu, sum, d), left_rows = __shfl_up_sync(0xffffffffu, sum_rows, d);
-                    if (lane >= d) sum += left, sum_rows += left_rows;
-                }
-                if (g < p.groups) s.begin[g] = run + sum - own, s.row[g] = rows + sum_rows - n;
-                run += __shfl_sync(0xffffffffu, sum, 31);
-                rows += __shfl_sync(0xffffffffu, sum_rows, 31);
+            // a lane has neighbouring groups, whose sums the warp adds up once
+            const int each = (p.groups + 31) >> 5, g0 = lane * each, g1 = min(g0 + each, p.groups);
+            int largest = s.largest;
+            if (kLayer) {
+#pragma unroll 1
+                for (int g = g0; g < g1; ++g) largest = max(largest, s.count[g]);
+                largest = __reduce_max_sync(0xffffffffu, largest);
+                if (lane == 0) s.largest = largest;
+            }
+            columns = widest(largest);
+            int own = 0, own_rows = 0;
+#pragma unroll 1
+            for (int g = g0; g < g1; ++g) own += parts_of(s.count[g], columns), own_rows += s.count[g];
+            int sum = own, sum_rows = own_rows;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int left = __shfl_up_sync(0xffffffffu, sum, d), left_rows = __shfl_up_sync(0xffffffffu, sum_rows, d);
+                if (lane >= d) sum += left, sum_rows += left_rows;
+            }
+            const int run = __shfl_sync(0xffffffffu, sum, 31);
+            sum -= own, sum_rows -= own_rows;
+#pragma unroll 1
+            for (int g = g0; g < g1; ++g) {
+                s.begin[g] = sum, s.row[g] = sum_rows;
+                sum += parts_of(s.count[g], columns), sum_rows += s.count[g];
             }
             // the height whose tiles take the fullest SM least: a whole box, or a lane a multiple of 8 from a piece on
             const int piece = kPieceRows / (kUp ? 2 : 1), h = lane == 31 ? p.full : 8 * (lane + 1);
@@ -311,7 +334,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     __syncthreads();
     if (kPair) cluster_sync();  // the other block's barriers are there
     tcgen05_after_sync();
-    if (kGrouped) height = s.height;
+    if (kGrouped) height = s.height, columns = widest(s.largest);
     const uint32_t tmem = s.tmem;
     const uint32_t full0 = shared_addr(s.full), empty0 = shared_addr(s.empty), sums_full0 = shared_addr(s.sums_full), sums_empty0 = shared_addr(s.sums_empty),
                    list_full0 = shared_addr(s.list_full), list_empty0 = shared_addr(s.list_empty), ring0 = shared_addr(ring);
