@@ -126,7 +126,7 @@ __device__ __forceinline__ uint4 exchange_packed(float (&v)[8], int lane) {
 // (The quick division gives 0 where the divisor is above 2^126: below -87, where silu is less than 1e-35.)
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + expf(-v)); }
 
-// Over all values at once: the choice inside a loop over them was two thirds of the epilogue (16384 rows of 1024 to 2048: 92 us where this takes
+// Over all values at once: the choice inside a loop over them was two thirds of the epilogue (16384 rows of 1024 to 2048: 92 us where this took
 // 62).
 template <int kCount>
 __device__ __forceinline__ void activate(float (&v)[kCount], int activation) {

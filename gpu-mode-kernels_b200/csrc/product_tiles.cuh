@@ -19,7 +19,7 @@
 // made a step of 64 take 1230 cycles where the weights' bytes take 700.)
 //
 // The second product of a layer leaves a row a pair, in fp32, and a launch of its own adds a token's rows up: tickets, by which the tile that
-// brings a token's last row adds them, took 3 us a tile (64 tokens of 2048, top-6 of 64: 146 us a layer where this takes 129).
+// brings a token's last row adds them, took 3 us a tile (64 tokens of 2048, top-6 of 64: 146 us a layer where this took 129).
 //
 // Roles of the twelve warps: 0 weights, 1 products, 2 rows, 3 the lists of rows, 4 to 11 the epilogue, two for each 32 lanes of the tensor
 // memory: every other 16 columns each.
@@ -58,7 +58,7 @@ constexpr int kMaxSplit = 8;
 constexpr int kTilesAhead = 64;
 // The tensor core cuts the sums it adds to: a sum of 7168 products came out 8e-6 off, of the 2-norm, where fp32 additions are 9e-7 off. For a result
 // of 32 bits a sum in tensor memory therefore is of about 512 of the inner length (5e-7 off), and the epilogue's threads add the parts up in
-// registers, which hold 128 columns. A sum of up to 896 is left whole (9e-7; 256 outputs of 7168, 16 rows, 6.5 us in parts and 5.9 at once), but for
+// registers, which hold 128 columns. A sum of up to 896 is left whole (9e-7; 256 outputs of 7168, 16 rows, took 6.5 us in parts and 5.9 at once), but for
 // SwiGLU, whose product doubles the error.
 constexpr int kSumBlocks = 8, kSumBlocksAtOnce = 14, kMaxColumns32 = 128;
 constexpr int kManyStep = 32;  // columns of a source in the slabs come in so many where there are many
@@ -730,8 +730,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 }
             };
             // The same for whole 16 columns and features in eights, with 16-byte stores: three exchanges between lanes turn a lane's 8 columns of a
-            // feature into 8 features of a column. (A store of two bytes for each value: 132 us for experts on slabs of 7000 rows of 2048
-            // where this takes 117.)
+            // feature into 8 features of a column. (A store of two bytes for each value took 132 us for experts on slabs of 7000 rows of
+            // 2048 where this took 117.)
             // (inner values: always)
             const bool wide_stores = kUp || (kOp != kLayerDown && p.wide_stores && (x.f & 7) == 0 && (x.height & 7) == 0);
             // where features f0 to f0 + 7 of column c go, and how many of them there are; none: 0

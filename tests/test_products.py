@@ -7,7 +7,7 @@ import torch
 
 import gpu_mode_kernels_b200 as pkg
 from gpu_mode_kernels_b200 import _lib
-from gpu_mode_kernels_b200.linear import check, linear
+from gpu_mode_kernels_b200.linear import DTYPES, check, linear
 from gpu_mode_kernels_b200.moe import expert_mlp, moe_layer, route, topk_gate
 from tests import product_oracle as O
 
@@ -305,6 +305,28 @@ def test_linear_strides_shapes_and_views():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,inputs", [(5, 2048), (70, 72), (600, 136), (1500, 520)])
+@pytest.mark.parametrize("outputs,stride", [(203, 208), (203, 211), (1000, 1016), (1001, 1008)])
+@pytest.mark.parametrize("activation,onto,out", [("none", False, None), ("gelu", False, None), ("silu", True, None), ("swiglu", False, None), ("swiglu", True, torch.float32),
+                                                 ("none", True, torch.float32)])
+def test_linear_results_in_rows_further_apart(tokens, inputs, outputs, stride, activation, onto, out):
+    """The C entry's strides: results beside what is not theirs, and onto the residual."""
+    g, dtype = generator(tokens, outputs, stride, activation), torch.float16 if stride % 3 else torch.bfloat16
+    rows = outputs * (2 if activation == "swiglu" else 1)
+    x, w, b = normal(g, tokens, inputs, dtype=dtype), normal(g, rows, inputs, std=inputs ** -0.5, dtype=dtype), normal(g, rows, dtype=dtype)
+    before = normal(g, tokens, stride, dtype=out or dtype)
+    dev, y = [t.to(DEV) for t in (x, w, b)], before.to(DEV)
+    at = y.data_ptr()
+    args = _lib.Linear(*(t.data_ptr() for t in dev), at if onto else 0, at, inputs, inputs, stride if onto else 0, stride, tokens, inputs, outputs,
+                       DTYPES[dtype], DTYPES[out or dtype], DTYPES[dtype], _lib.ACTIVATION[activation])
+    assert _lib.load().a2a_linear(C.byref(args), _lib.current_stream()) == 0
+    check()
+    value, bound = O.linear(x, w, b, activation, before[:, :outputs] if onto else None, out or dtype)
+    O.assert_within(y[:, :outputs], value, bound)
+    assert torch.equal(y[:, outputs:].cpu(), before[:, outputs:])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [1, 30, 300])
 def test_linear_many_outputs(tokens):
     """As many as a vocabulary has, past the sizes that a layer's matrices have."""
@@ -478,6 +500,39 @@ def test_experts_on_slabs(local, world, capacity, hidden, inner, dtype, in_place
     behind = torch.arange(capacity)[None, None] >= n.t()[..., None]
     rows[behind] = float("nan")  # what an earlier call left
     check_slabs(rows, n, gate_up, down, in_place)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden,inner", [(1416, 8), (8, 2056)])
+def test_more_tiles_than_a_block_has_room_for(hidden, inner):
+    """1024 experts of a row each, of which a block gets 80 to 230 tiles: in its table, and behind the end of that."""
+    g = generator(hidden, inner)
+    gate_up, down = some_experts(g, 1024, hidden, inner, torch.bfloat16)
+    x, w = normal(g, 32, hidden, dtype=torch.bfloat16), torch.softmax(normal(g, 32, 32), 1)
+    check_layer(x, torch.randperm(1024, generator=g).view(32, 32).to(torch.int32), w, gate_up, down)
+    check_slabs(normal(g, 1024, 1, 1, hidden, dtype=torch.bfloat16), torch.ones(1, 1024, dtype=torch.int64), gate_up, down)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden", [64, 264, 1032])
+def test_experts_results_off_sixteen_bytes(hidden):
+    g = generator(hidden, 3)
+    gate_up, down = some_experts(g, 3, hidden, 40, torch.float16)
+    rows, n = normal(g, 3, 2, 70, hidden, dtype=torch.float16), torch.tensor([[70, 0, 33], [1, 64, 7]])
+    space = torch.full((rows.numel() + 3,), 3.0, dtype=torch.float16, device=DEV)
+    out = space[3:].view(rows.shape)
+    counts = torch.zeros(2, 4, 3, dtype=torch.int32)
+    counts[:, 0] = n
+    expert_mlp(rows.to(DEV), counts.to(DEV), gate_up.to(DEV), down.to(DEV), out=out)
+    check()
+    for l in range(3):
+        for s in range(2):
+            v = int(n[s, l])
+            if v:
+                value, bound = O.expert(rows[l, s, :v], gate_up[l], down[l], rows.dtype)
+                O.assert_within(out[l, s, :v], value, O.rounded(value, bound, rows.dtype))
+            assert bool((out[l, s, v:] == 3.0).all())
+    assert bool((space[:3] == 3.0).all())
 
 
 @pytest.mark.gpu
