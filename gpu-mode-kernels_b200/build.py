@@ -24,6 +24,7 @@ HEADERS = [os.path.join(CSRC, "a2a_kernels.cuh"), os.path.join(CSRC, "a2a_pipe.c
            os.path.join(CSRC, "a2a_solo.cuh"),
            os.path.join(CSRC, "a2a_device.cuh"),
            os.path.join(CSRC, "product_device.cuh"), os.path.join(CSRC, "product_tiles.cuh"),
+           os.path.join(CSRC, "product_shares.h"),
            os.path.join(ROOT, "include", "a2a.h")]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
          "-I", os.path.join(ROOT, "include"), "-I", CSRC]

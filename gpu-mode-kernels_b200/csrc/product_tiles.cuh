@@ -34,6 +34,7 @@
 #pragma once
 
 #include "product_device.cuh"
+#include "product_shares.h"
 
 namespace {
 
@@ -396,20 +397,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         __syncthreads();
     }
     auto tile_at = [&](int n) { return kGrouped && n < kTilesAhead ? s.tile[n] : tile_of(tile0 + n * tile_step); };
-    // columns of a tile's product, and of those the ones that block `of` of the pair copies
+    // columns of a tile's product, and of those the ones that block `of` copies, in eights
     auto product_columns = [&](const Tile& x) {
         if (kOne && kPair) return columns;
         return ((kOp == kLayerUp && !p.sorted ? p.tokens : x.columns) + kColumnStep - 1) / kColumnStep * kColumnStep;
     };
-    auto columns_of = [&](const Tile& x, int of, int& from) {
-        if (!kPair) {
-            from = 0;
-            return x.columns;
-        }
-        const int half = product_columns(x) / 2;
-        from = of * half;
-        return max(0, min(half, x.columns - from));
-    };
+    auto columns_of = [&](const Tile& x, int of, int& from) { return copied_columns(x.columns, product_columns(x), kBlocks, of, &from); };
     // kLayer*: a pair's expert, -1 for none
     auto expert_of = [&](int pair) {
         if (pair < kCached) return (int)s.expert[pair];
@@ -500,11 +493,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                 if (kOne) columns_of(x, side, from);
                 if (runs) {
                     bytes = 0;
-                    for (int of = 0; of < kBlocks; ++of) {
-                        const int n8 = (columns_of(x, of, from) + 7) & ~7, size = n8 >= 64 ? 64 : n8 >= 32 ? 32 : 8;
-                        bytes += (n8 + size - 1) / size * size * kRowBytes;
-                    }
-                    run = (columns_of(x, side, from) + 7) & ~7;
+                    for (int of = 0; of < kBlocks; ++of) bytes += boxed_rows(columns_of(x, of, from)) * kRowBytes;
+                    run = columns_of(x, side, from);
                 } else if (kOp == kSlabUp) {
                     if (!barrier_wait(list_full0 + 8 * (n & 1), (n >> 1) & 1, &s.gave_up)) goto rows_done;
                     wide_boxes = s.boxes[n & 1][0], some_boxes = s.boxes[n & 1][1], boxes = s.boxes[n & 1][2];
@@ -597,7 +587,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                         const int row = row_at(c, valid);
                         s.list[buffer][c] = valid ? row : -1;
                     }
-                    // Lane i looks at columns 8 i to 8 i + 7: where their run begins and ends, and whether a box begins there.
+                    // Lane i looks at columns 8 i to 8 i + 7: where their run begins and ends, and whether a box begins there. (The columns that a second
+                    // block copies for nothing are of rows of any kind, or behind the last one, which come as zeros.)
                     int box_rows = 0;
                     for (int of = 0; of < kBlocks; ++of) {
                         int from;
