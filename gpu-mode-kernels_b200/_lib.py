@@ -121,6 +121,7 @@ SIGNATURES = {
     "a2a_experts_workspace": (C.c_size_t, [_I, _I, _I, _I]),
     "a2a_experts": (_I, [C.POINTER(Experts), _VP]),
     "a2a_product_status": (_I, [C.POINTER(C.c_int32)]),
+    "a2a_product_word": (_VP, [_I]),
     "a2a_status": (_I, [_VP, C.POINTER(Status)]),
     "a2a_status_clear": (_I, [_VP]),
     "a2a_status_peek": (_I, [_VP]),
@@ -200,6 +201,12 @@ def host():
 def current_stream() -> int:
     """The current CUDA stream of the current device, as the C ABI takes it."""
     return _raw_stream(torch.cuda.current_device())
+
+
+def product_error(device: int) -> int:
+    """The code that a product (linear.py, moe.py) on ``device`` has recorded, 0 for none: a read of mapped host memory."""
+    word = load().a2a_product_word(device)
+    return C.c_int32.from_address(word).value if word else 0
 
 
 def strerror(code: int) -> str:

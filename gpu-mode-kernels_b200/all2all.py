@@ -20,6 +20,7 @@ import torch.distributed as dist
 
 from . import _lib, moe
 from ._lib import A2AError, Config, Status  # noqa: F401
+from .linear import check as check_products
 from .task import MoEConfig, input_t, output_t
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
@@ -31,6 +32,8 @@ def _ptr(t: Optional[torch.Tensor]) -> C.c_void_p:
 
 class A2AContext:
     """State of one rank for one (config, process group): buffers, peer mappings, flags."""
+
+    _products = False  # whether ``experts`` has been called
 
     def __init__(self, cfg: MoEConfig, rank: int, world_size: int, *, device: Optional[int] = None,
                  payload: str = "direct", schedule: str = "phased", combine: str = "pull",
@@ -145,11 +148,13 @@ class A2AContext:
     def experts(self, gate_up: torch.Tensor, down: torch.Tensor) -> None:
         """This rank's experts (``moe.expert_mlp``) on the rows that ``dispatch_recv`` left, in place, then ``expert_done``: the
         real expert op in the place of ``expert_placeholder``.  ``gate_up`` is ``[local experts, 2 * inner, hidden]``, ``down``
-        ``[local experts, hidden, inner]``, in the type of the rows, on this rank's GPU."""
+        ``[local experts, hidden, inner]``, in the type of the rows, on this rank's GPU.  ``check`` and ``peek`` then look at what the products
+        on this GPU have recorded, too."""
         if self.schedule != "phased" or self._chunked:
             raise A2AError(_lib.A2A_ERR_STATE, "experts run between the phases of the phased schedule, of calls in one chunk")
         with torch.cuda.device(self.device_index):
             rows, counts = self.expert_buffers()
+            self._products = True
             moe.expert_mlp(rows, counts, gate_up, down)
             self.expert_done()
 
@@ -285,15 +290,18 @@ class A2AContext:
         return s
 
     def check(self) -> None:
-        """Raise if a kernel of this context has recorded an error."""
+        """Raise if a kernel of this context has recorded an error, or a product on this GPU after ``experts`` (which is then forgotten)."""
         s = self.status()
         if s.code != 0:
             raise A2AError(s.code, f"{_lib.strerror(s.code)} (rank {s.rank}, peer {s.peer}, phase {s.phase}, "
                                    f"call {s.epoch}, detail {s.detail})")
+        if self._products:
+            with torch.cuda.device(self.device_index):
+                check_products()
 
     def peek(self) -> int:
-        """The recorded error code (0 = none) without any CUDA call: a read of mapped host memory."""
-        return self.lib.a2a_status_peek(self._h)
+        """The recorded error code (0 = none), of a product on this GPU after ``experts``, too, without any CUDA call: reads of mapped host memory."""
+        return self.lib.a2a_status_peek(self._h) or (self._products and _lib.product_error(self.device_index)) or 0
 
     def raise_and_clear_if_failed(self) -> None:
         """What the plugin entry does before every call: if an earlier call recorded an error,
@@ -301,6 +309,8 @@ class A2AContext:
         if self.peek() == 0:
             return
         s = self.status()
+        if s.code == 0 and self._products:
+            return self.check()
         self.clear_status()
         raise A2AError(s.code, f"an earlier call failed: {_lib.strerror(s.code)} (rank {s.rank}, peer {s.peer}, "
                                f"phase {s.phase}, call {s.epoch}, detail {s.detail}); the status has been cleared")

@@ -3,6 +3,7 @@
 // All of them are product_tiles.cuh's kernel.
 #include <algorithm>
 #include <atomic>
+#include <cstring>
 
 #include "product_device.cuh"
 #include "product_tiles.cuh"
@@ -58,18 +59,49 @@ int weights_map(CUtensorMap* map, int dtype, const void* p, int groups, int feat
                : A2A_ERR_CONFIG;
 }
 
-int sm_count(int* sms) {
-    static std::atomic<int> known[64];
+constexpr int kDevices = 64;
+
+// A word a device, on a page of mapped host memory that the process's first call asks for, and keeps: kernels record there that a wait ran out, and the
+// host looks without a CUDA call. A first call may be a captured one, in which nothing is allocated unless the thread says that it may.
+int32_t* error_word(int device) {
+    static std::atomic<int32_t*> known{nullptr};
+    if (device < 0 || device >= kDevices) return nullptr;
+    int32_t* words = known.load(std::memory_order_acquire);
+    if (words == nullptr) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+        void* page = nullptr;
+        int32_t* fresh = nullptr;
+        if (cudaHostAlloc(&page, kDevices * sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
+            fresh = static_cast<int32_t*>(page);
+            memset(fresh, 0, kDevices * sizeof(int32_t));
+            if (known.compare_exchange_strong(words, fresh, std::memory_order_acq_rel)) words = fresh;
+            else cudaFreeHost(page);  // another thread was first
+        } else {
+            cudaGetLastError();
+        }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+    return words == nullptr ? nullptr : words + device;
+}
+
+// What a call needs of the current device: its SMs, and its word for errors, which is 0 or the call's answer.
+struct Ready {
+    int sms;
+    int32_t* error;
+};
+int get_ready(Ready* r) {
+    static std::atomic<int> known[kDevices];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return -(int)e;
-    int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
-    if (n == 0) {
-        if ((e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return -(int)e;
-        if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    if ((r->error = error_word(dev)) == nullptr) return -(int)cudaErrorMemoryAllocation;
+    r->sms = known[dev].load(std::memory_order_relaxed);
+    if (r->sms == 0) {
+        if ((e = cudaDeviceGetAttribute(&r->sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return -(int)e;
+        known[dev].store(r->sms, std::memory_order_relaxed);
     }
-    *sms = n;
-    return A2A_OK;
+    return *reinterpret_cast<volatile int32_t*>(r->error);
 }
 
 // Lets the kernel have its shared memory on the current device.
@@ -196,14 +228,15 @@ DensePlan dense_plan(const a2a_linear_args& a, bool paired, int sms) {
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 template <TilesOp kOp, typename T>
-int linear_of(const a2a_linear_args& a, int sms, cudaStream_t st) {
+int linear_of(const a2a_linear_args& a, const Ready& gpu, cudaStream_t st) {
     const bool paired = a.activation == A2A_ACT_SWIGLU;
     TilesParams p{};
+    p.error = gpu.error;
     p.inner = a.inputs, p.features = a.outputs, p.paired = paired, p.groups = 1, p.tokens = a.tokens;
     p.activation = a.activation, p.bias_fp32 = a.bias_dtype == A2A_DTYPE_FP32;
     p.bias = a.bias, p.residual = a.residual, p.residual_stride = a.residual_stride, p.y = a.y, p.y_stride = a.y_stride;
     p.wide_stores = a.y_stride % 8 == 0 && aligned(a.y) && (a.residual == nullptr || (a.residual_stride % 8 == 0 && aligned(a.residual)));
-    const DensePlan plan = dense_plan<kOp, T>(a, paired, sms);
+    const DensePlan plan = dense_plan<kOp, T>(a, paired, gpu.sms);
     p.columns = plan.columns, p.full = plan.height, p.split = plan.split;
     int rc = weights_map(&p.weights, a.dtype, a.weight, 1, a.outputs, paired, a.inputs, a.weight_stride, plan.height);
     if (rc == A2A_OK) rc = rows_map(&p.rows, a.dtype, a.x, a.tokens, a.inputs, a.x_stride, plan.pair ? p.columns / 2 : p.columns);
@@ -213,7 +246,7 @@ int linear_of(const a2a_linear_args& a, int sms, cudaStream_t st) {
         return launch_tiles<kOp, T, kPairs>(p, 2 * std::min(tiles, most_clusters<kOp, T, kPairs>(2)), 2, st);
     }
     const int tiles = parts_of(a.outputs, plan.height) * parts_of(a.tokens, plan.columns);
-    return plan.split > 1 ? launch_tiles<kOp, T, kCuts>(p, tiles * plan.split, plan.split, st) : launch_tiles<kOp, T>(p, std::min(tiles, sms), 1, st);
+    return plan.split > 1 ? launch_tiles<kOp, T, kCuts>(p, tiles * plan.split, plan.split, st) : launch_tiles<kOp, T>(p, std::min(tiles, gpu.sms), 1, st);
 }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -250,10 +283,11 @@ int run_maps(TilesParams& p, int dtype, const void* rows, long long count) {
 }
 
 template <typename T>
-int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
+int layer_of(const a2a_layer_args& a, const Ready& gpu, cudaStream_t st) {
     uint8_t* const space = static_cast<uint8_t*>(a.workspace);
     const LayerSpace at = layer_space(a.tokens, a.topk, a.hidden_dim, a.inner);
     TilesParams p{};
+    p.error = gpu.error;
     p.groups = a.experts, p.tokens = a.tokens, p.topk = a.topk, p.indices = a.topk_idx, p.weights_of = a.topk_weights;
     p.hidden = space, p.parts = reinterpret_cast<float*>(space + at.parts);
     p.columns = kMaxColumns;
@@ -266,11 +300,11 @@ int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
         SortParams sort{a.x, a.topk_idx, p.parts, a.tokens, a.topk, a.experts, a.hidden_dim * 2};
         if (rc == A2A_OK) rc = launch(reinterpret_cast<const void*>(&layer_rows_kernel), a.tokens * a.topk, kSortThreads, 0, 1, &sort, st);
     }
-    if (rc == A2A_OK) rc = launch_tiles<kLayerUp, T>(p, sms, 1, st);
+    if (rc == A2A_OK) rc = launch_tiles<kLayerUp, T>(p, gpu.sms, 1, st);
     if (rc != A2A_OK) return rc;
     rc = expert_maps(p, a.dtype, a.down, a.experts, a.hidden_dim, false, a.inner);
     if (rc == A2A_OK) rc = run_maps(p, a.dtype, p.hidden, (long long)a.tokens * a.topk);
-    if (rc == A2A_OK) rc = launch_tiles<kLayerDown, T>(p, sms, 1, st);
+    if (rc == A2A_OK) rc = launch_tiles<kLayerDown, T>(p, gpu.sms, 1, st);
     if (rc != A2A_OK) return rc;
     SumParams sum{p.parts, a.topk_idx, a.residual, a.y, a.topk, a.experts, a.hidden_dim};
     return launch(reinterpret_cast<const void*>(&layer_sum_kernel<T>), dim3(a.tokens, parts_of(a.hidden_dim, 4 * kSumThreads)), kSumThreads, 0, 1, &sum, st);
@@ -280,9 +314,10 @@ int layer_of(const a2a_layer_args& a, int sms, cudaStream_t st) {
 long long inner_rows(int local_experts, int world, int capacity) { return (long long)local_experts * world * ((capacity + kManyStep - 1) & -kManyStep); }
 
 template <typename T>
-int experts_of(const a2a_experts_args& a, int sms, cudaStream_t st) {
+int experts_of(const a2a_experts_args& a, const Ready& gpu, cudaStream_t st) {
     const long long rows = (long long)a.local_experts * a.world * a.capacity;
     TilesParams p{};
+    p.error = gpu.error;
     p.groups = a.local_experts, p.counts = a.counts, p.world = a.world, p.capacity = a.capacity, p.hidden = a.workspace;
     p.columns = kMaxColumns;
     int rc = expert_maps(p, a.dtype, a.gate_up, a.local_experts, a.inner, true, a.hidden_dim);
@@ -311,13 +346,13 @@ extern "C" int a2a_linear(const a2a_linear_args* args, void* stream) {
     if (a.x == nullptr || a.weight == nullptr || a.y == nullptr || !aligned(a.x) || !aligned(a.weight)) return A2A_ERR_CONFIG;
     if (a.x_stride < a.inputs || a.x_stride % 8 != 0 || a.weight_stride < a.inputs || a.weight_stride % 8 != 0) return A2A_ERR_CONFIG;
     if (a.y_stride < a.outputs || (a.residual != nullptr && a.residual_stride < 0)) return A2A_ERR_CONFIG;
-    int sms = 0;
-    const int rc = sm_count(&sms);
+    Ready gpu{};
+    const int rc = get_ready(&gpu);
     if (rc != A2A_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (a.out_dtype == A2A_DTYPE_FP32)
-        return a.dtype == A2A_DTYPE_BF16 ? linear_of<kDense32, __nv_bfloat16>(a, sms, st) : linear_of<kDense32, __half>(a, sms, st);
-    return a.dtype == A2A_DTYPE_BF16 ? linear_of<kDense, __nv_bfloat16>(a, sms, st) : linear_of<kDense, __half>(a, sms, st);
+        return a.dtype == A2A_DTYPE_BF16 ? linear_of<kDense32, __nv_bfloat16>(a, gpu, st) : linear_of<kDense32, __half>(a, gpu, st);
+    return a.dtype == A2A_DTYPE_BF16 ? linear_of<kDense, __nv_bfloat16>(a, gpu, st) : linear_of<kDense, __half>(a, gpu, st);
 }
 
 extern "C" size_t a2a_layer_workspace(int num_tokens, int experts_per_token, int hidden_dim, int inner) {
@@ -336,11 +371,11 @@ extern "C" int a2a_layer(const a2a_layer_args* args, void* stream) {
         return A2A_ERR_CONFIG;
     if (!aligned(a.x) || !aligned(a.gate_up) || !aligned(a.down) || reinterpret_cast<uintptr_t>(a.workspace) % 256 != 0) return A2A_ERR_CONFIG;
     if (a.workspace_bytes < layer_space(a.tokens, a.topk, a.hidden_dim, a.inner).end) return A2A_ERR_CAPACITY;
-    int sms = 0;
-    const int rc = sm_count(&sms);
+    Ready gpu{};
+    const int rc = get_ready(&gpu);
     if (rc != A2A_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    return a.dtype == A2A_DTYPE_BF16 ? layer_of<__nv_bfloat16>(a, sms, st) : layer_of<__half>(a, sms, st);
+    return a.dtype == A2A_DTYPE_BF16 ? layer_of<__nv_bfloat16>(a, gpu, st) : layer_of<__half>(a, gpu, st);
 }
 
 extern "C" size_t a2a_experts_workspace(int local_experts, int world_size, int capacity, int inner) {
@@ -357,19 +392,21 @@ extern "C" int a2a_experts(const a2a_experts_args* args, void* stream) {
         return A2A_ERR_CONFIG;
     if (!aligned(a.rows) || !aligned(a.gate_up) || !aligned(a.down) || reinterpret_cast<uintptr_t>(a.workspace) % 256 != 0) return A2A_ERR_CONFIG;
     if (a.workspace_bytes < a2a_experts_workspace(a.local_experts, a.world, a.capacity, a.inner)) return A2A_ERR_CAPACITY;
-    int sms = 0;
-    const int rc = sm_count(&sms);
+    Ready gpu{};
+    const int rc = get_ready(&gpu);
     if (rc != A2A_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    return a.dtype == A2A_DTYPE_BF16 ? experts_of<__nv_bfloat16>(a, sms, st) : experts_of<__half>(a, sms, st);
+    return a.dtype == A2A_DTYPE_BF16 ? experts_of<__nv_bfloat16>(a, gpu, st) : experts_of<__half>(a, gpu, st);
 }
+
+extern "C" int32_t* a2a_product_word(int device) { return error_word(device); }
 
 extern "C" int a2a_product_status(int32_t* code) {
     if (code == nullptr) return A2A_ERR_CONFIG;
-    cudaError_t e = cudaDeviceSynchronize();
-    int zero = 0, got = 0;
-    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&got, g_product_error, sizeof(int));
-    if (e == cudaSuccess && got != 0) e = cudaMemcpyToSymbol(g_product_error, &zero, sizeof(int));
-    *code = got;
+    Ready gpu{};
+    const int rc = get_ready(&gpu);
+    if (rc < 0) return rc;
+    const cudaError_t e = cudaDeviceSynchronize();
+    *code = __atomic_exchange_n(gpu.error, A2A_OK, __ATOMIC_ACQ_REL);
     return e == cudaSuccess ? A2A_OK : -(int)e;
 }

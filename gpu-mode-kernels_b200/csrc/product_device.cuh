@@ -19,9 +19,6 @@ namespace {
 // what the step moved.)
 constexpr long long kWaitCycles = 4000000000ll;
 
-// Set by a kernel whose wait ran out; read and cleared by a2a_product_status.
-__device__ int g_product_error;
-
 // ---- element types -----------------------------------------------------------------------------
 template <typename T>
 struct Element;

@@ -96,6 +96,7 @@ struct TilesParams {
     // kSlab*
     const int* counts;
     int world, capacity;
+    int* error;  // mapped host memory: where a wait that ran out is recorded
 };
 
 // a / b for a >= 0, b > 0. A block works out a dozen of them, one after the other, before its first copy is on its way: an integer division is
@@ -903,7 +904,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
         // copies and products in flight end in less than this
         const long long begin = clock64();
         while (clock64() - begin < 2000000) __nanosleep(1000);
-        if (tid == 0) atomicExch(&g_product_error, A2A_ERR_TIMEOUT);
+        if (tid == 0) {
+            *reinterpret_cast<volatile int*>(p.error) = A2A_ERR_TIMEOUT;
+            __threadfence_system();
+        }
         __syncthreads();
     }
     if (warp == 1) tmem_free<kPair>(tmem, kTmemColumns);

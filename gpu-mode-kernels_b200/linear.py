@@ -21,6 +21,14 @@ def refuse(message: str):
     raise _lib.A2AError(_lib.A2A_ERR_CONFIG, message)
 
 
+def failed(code: int):
+    """Raise for a status code of a product."""
+    if code == _lib.A2A_ERR_TIMEOUT:
+        raise _lib.A2AError(code, "a wait inside an earlier product on this GPU ran out, and what it left is not valid; nothing has been launched now "
+                                  "(linear.check() clears this)")
+    _lib.check(code)
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the bytes from the first to the last element of two strided tensors meet."""
     if a.numel() == 0 or b.numel() == 0:
@@ -38,11 +46,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     (by the error function), ``"silu"``, or ``"swiglu"``: ``weight`` ``[2 * outputs, inputs]`` holds gate rows before up rows and the result is
     ``silu(gate) * up``.  ``bias`` has the weight's rows, in its type or fp32; ``residual`` the result's shape and type.  ``out_dtype``: the
     type of ``x`` (default) or ``torch.float32``.  Sums and the epilogue are fp32, with one rounding at the end.  For inference: no gradient is
-    recorded.
+    recorded.  Raises where an earlier product on this GPU has recorded an error (``check``).
     """
     out = _lib.host().linear(x, weight, bias, activation, residual, out_dtype)
     if out is not None:
-        return out if type(out) is not int else _lib.check(out)
+        return out if type(out) is not int else failed(out)
     # something is wrong, or unusual: look again, one thing at a time
     if x.dtype not in _SIXTEEN or not x.is_cuda or x.dim() < 1:
         refuse(f"x must be a bf16 or fp16 CUDA tensor [..., inputs], got {x.dtype} {tuple(x.shape)} on {x.device}")
@@ -95,12 +103,15 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
                        DTYPES[x.dtype if bias is None else bias.dtype], _lib.ACTIVATION[activation])
     rc = _lib.load().a2a_linear(C.byref(args), _lib.current_stream())
     if rc != 0:
-        _lib.check(rc)
+        failed(rc)
     return y
 
 
 def check() -> None:
-    """Raise if a product on the current device has recorded an error since the last look (synchronises the device)."""
+    """Raise if a product (``linear``, ``moe_layer``, ``expert_mlp``) on the current device has recorded an error since the last look, and forget it
+    (synchronises the device).  A wait inside a kernel that ran out is recorded when it does, after the call has returned: without this the next product
+    raises, and launches nothing; replays of a captured graph do not look."""
     code = C.c_int32()
     _lib.check(_lib.load().a2a_product_status(C.byref(code)))
-    _lib.check(code.value)
+    if code.value != 0:
+        raise _lib.A2AError(code.value, "a wait inside a product on this GPU ran out: what it left is not valid; the record has been cleared")

@@ -17,7 +17,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .linear import DTYPES, _overlap, linear, refuse
+from .linear import DTYPES, _overlap, failed, linear, refuse
 
 _SIXTEEN = (torch.bfloat16, torch.float16)
 
@@ -94,10 +94,11 @@ def moe_layer(x: torch.Tensor, indices: torch.Tensor, weights: torch.Tensor, gat
     index outside the experts marks none (a padded token's row is its residual, or 0); the same expert twice counts twice.  Sums are fp32;
     an expert's inner values are rounded to the type, since the second product takes 16-bit operands, and the result once.
     More tokens go through ``A2AContext`` with ``experts`` between dispatch and combine.  For inference: no gradient is recorded.
+    Raises where an earlier product on this GPU has recorded an error (``linear.check``).
     """
     out = _lib.host().layer(x, indices, weights, gate_up, down, residual)
     if out is not None:
-        return out if type(out) is not int else _lib.check(out)
+        return out if type(out) is not int else failed(out)
     # something is wrong, or unusual: look again, one thing at a time
     if x.dtype not in _SIXTEEN or not x.is_cuda or x.dim() != 2 or not x.is_contiguous():
         refuse(f"x must be a contiguous bf16 or fp16 CUDA tensor [tokens, hidden], got {x.dtype} {tuple(x.shape)} on {x.device}")
@@ -130,7 +131,7 @@ def moe_layer(x: torch.Tensor, indices: torch.Tensor, weights: torch.Tensor, gat
                       tokens, topk, experts, hidden, inner, DTYPES[x.dtype])
     rc = lib.a2a_layer(C.byref(args), _lib.current_stream())
     if rc != 0:
-        _lib.check(rc)
+        failed(rc)
     return y
 
 
@@ -140,7 +141,8 @@ def expert_mlp(rows: torch.Tensor, counts: torch.Tensor, gate_up: torch.Tensor, 
     ``A2AContext.expert_buffers`` gives them; row i of slab (l, s) is valid for ``i < counts[s, 0, l]``.
 
     The results go where the rows are, or to ``out`` of the same shape and type, which is returned; what lies behind a slab's
-    valid rows is left as it is.  Sums are fp32; inner values and results are rounded to the type of the rows.
+    valid rows is left as it is.  Sums are fp32; inner values and results are rounded to the type of the rows.  Raises where an earlier product
+    on this GPU has recorded an error (``linear.check``).
     """
     if rows.dtype not in _SIXTEEN or not rows.is_cuda or rows.dim() != 4 or not rows.is_contiguous():
         refuse(f"rows must be a contiguous bf16 or fp16 CUDA tensor [local experts, world, capacity, hidden], got {rows.dtype} "
@@ -170,5 +172,5 @@ def expert_mlp(rows: torch.Tensor, counts: torch.Tensor, gate_up: torch.Tensor, 
                         space.numel(), local, world, capacity, hidden, inner, DTYPES[rows.dtype])
     rc = lib.a2a_experts(C.byref(args), _lib.current_stream())
     if rc != 0:
-        _lib.check(rc)
+        failed(rc)
     return out

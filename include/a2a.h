@@ -349,7 +349,8 @@ size_t a2a_symmetric_bytes(a2a_ctx* ctx);
 /* ---- The layer around the all-to-all: gate, experts, dense products -----------------------------------
  * No counterpart in the reference, whose experts are a placeholder (reference.py:262) and whose routing is drawn at random
  * (reference.py:33-43).  None of these calls needs a context; they run on the current device, allocate nothing, keep nothing from
- * one call for the next and never synchronise; workspaces are the caller's, 256-byte aligned, of the size the *_workspace function
+ * one call for the next and never synchronise (but for a page of host
+ * memory for a2a_product_word, of which the process's first call asks for); workspaces are the caller's, 256-byte aligned, of the size the *_workspace function
  * gives, and not shared by calls that may run at the same time.  Element types are A2A_DTYPE_BF16 and
  * A2A_DTYPE_FP16; sums are fp32.  Values too large for fp16 become infinite, in an expert's inner values too. */
 enum { A2A_DTYPE_FP32 = 2 };
@@ -420,9 +421,13 @@ typedef struct a2a_experts_args {
 size_t a2a_experts_workspace(int local_experts, int world_size, int capacity, int inner);
 int a2a_experts(const a2a_experts_args* args, void* stream);
 
-/* What the products on the current device recorded since the last call: A2A_OK, or A2A_ERR_TIMEOUT where a wait inside a kernel ran out
- * (its outputs are not valid).  Synchronises the device. */
+/* What the products (a2a_linear, a2a_layer, a2a_experts) on the current device recorded since the last call of this one: A2A_OK, or
+ * A2A_ERR_TIMEOUT where a wait inside a kernel ran out (the outputs of that product, and of what took them, are not valid).  Synchronises the device,
+ * and forgets what it answers.  Until then the products on this device launch nothing and answer with the recorded code themselves. */
 int a2a_product_status(int32_t* code);
+/* The word in mapped host memory that the products on `device` record that code in, the same one for as long as the process runs: a look at it
+ * needs no CUDA call, and may be ahead of a kernel that still runs.  NULL where there is no memory of that kind, or no such device (0 to 63). */
+int32_t* a2a_product_word(int device);
 
 #ifdef __cplusplus
 }
