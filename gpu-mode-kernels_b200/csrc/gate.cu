@@ -145,9 +145,29 @@ __global__ void __launch_bounds__(kThreads) gate_kernel(const GateParams p) {
             best_of(best, at, value);
         }
     }
+    // The ratio of scores does not hang on how small they are: where the chosen ones come to less than 2^-64 they are looked at again, in 64 bits and
+    // relative to the largest logit among them (1 / (1 + exp(-l)) is 0 in 32 bits from -89 on; next to a larger sum what is lost there weighs
+    // less than 2^-62).
+    if (p.renormalize && sum < (V)(1.0 / 18446744073709551616.0)) {
+        const double l = lane < p.topk ? (double)as_float(row[chosen]) : -INFINITY;
+        double most = l;
+        for (int d = 16; d > 0; d >>= 1) {
+            const double other = __shfl_xor_sync(0xffffffffu, most, d);
+            most = other > most ? other : most;
+        }
+        // (chosen from a row of nothing but -inf: zeros)
+        double r = most == -INFINITY ? 0.0 : exp(l - most);
+        if (p.sigmoid) r /= 1.0 + exp(l);
+        const double all = warp_sum(r);
+        if (lane < p.topk) {
+            p.indices[(size_t)token * p.topk + lane] = chosen;
+            p.weights[(size_t)token * p.topk + lane] = (float)(all == 0.0 ? 0.0 : r / all * (double)p.scale);
+        }
+        return;
+    }
     if (lane < p.topk) {
         V w = mine;
-        if (p.renormalize) w = sum == 0 ? (V)0 : w / sum;
+        if (p.renormalize) w = w / sum;
         p.indices[(size_t)token * p.topk + lane] = chosen;
         p.weights[(size_t)token * p.topk + lane] = (float)(w * (V)p.scale);
     }

@@ -28,7 +28,7 @@ def topk_gate(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Opt
 
     Scores are the softmax or the sigmoid of the logits.  The k largest logits are chosen, or with ``bias`` ``[experts]`` fp32 the
     k largest ``score + bias`` (in 64 bits; the bias is not part of the weights), in descending order, ties to the lowest index.  Weights are the
-    chosen scores, divided by their sum with ``renormalize`` (0 where that is 0), times ``scale``.  A logit of -inf excludes an expert while k
+    chosen scores, divided by their sum with ``renormalize`` (however small that is; 0 where all chosen logits are -inf), times ``scale``.  A logit of -inf excludes an expert while k
     others are there; a row of nothing else gets weights 0 with softmax.  NaN ranks first, and the weights of its row are NaN with softmax.
     For inference: no gradient is recorded.
     """

@@ -362,7 +362,7 @@ enum { A2A_MAX_PRODUCT = 65536, A2A_MAX_OUTPUTS = 1 << 24, A2A_MAX_ROWS = 1 << 3
 /* Gate: indices and weights [tokens, topk] from logits [tokens, experts] (rows `stride` apart), as a2a_route and a2a_forward take
  * them.  score s = softmax or sigmoid of the logits; chosen are the topk largest logits, or, with a bias [experts], the largest s + bias
  * (in 64 bits), in descending order, ties to the lowest index; a NaN ranks above everything.  weight = scale * s, divided by the sum of the
- * chosen s if renormalize is not zero (0 where that sum is 0, as for a row of nothing but -inf with softmax).  -inf excludes an
+ * chosen s if renormalize is not zero, however small that is (0 where all chosen logits are -inf).  -inf excludes an
  * expert as long as topk others are there. */
 typedef struct a2a_gate_args {
     const void* logits; /* dtype: any of the three */
