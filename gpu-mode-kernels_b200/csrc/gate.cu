@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kThreads) gate_kernel(const GateParams p) {
         if (sizeof(V) == 4 && e < p.experts) key[j] = key_of(score[j]);
         if constexpr (sizeof(V) == 8) bias[j] = e < p.experts ? p.bias[e] : 0.0f;
     }
-    // a logit of -inf is behind all others whatever its bias: a bit an expert
+    // a logit of -inf is behind all others whatever its bias and theirs, of -inf too: a bit an expert
     uint32_t excluded = 0;
     if constexpr (sizeof(V) == 8) {
 #pragma unroll kOwn
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) gate_kernel(const GateParams p) {
         score[j] *= share;
         const int e = 32 * j + lane;
         if constexpr (sizeof(V) == 8)
-            if (e < p.experts) key[j] = key_of(excluded >> j & 1 ? (V)-INFINITY : score[j] + (V)bias[j]);
+            if (e < p.experts) key[j] = excluded >> j & 1 ? (Key)1 : key_of(score[j] + (V)bias[j]);
     }
 
     // this lane's best, the lowest index among equals
