@@ -57,11 +57,10 @@ constexpr int kSpreadTokens = 64;  // 40 to 100 tokens take the same either way
 constexpr int kPieceRows = 32;  // operand rows of a box of a tile that is less than full
 constexpr int kMaxSplit = 8;
 constexpr int kTilesAhead = 64;
-// The tensor core cuts the sums it adds to: a sum of 7168 products came out 8e-6 off, of the 2-norm, where fp32 additions are 9e-7 off. For a result
-// of 32 bits a sum in tensor memory therefore is of about 512 of the inner length (5e-7 off), and the epilogue's threads add the parts up in
-// registers, which hold 128 columns. A sum of up to 896 is left whole (9e-7; 256 outputs of 7168, 16 rows, took 6.5 us in parts and 5.9 at once), but for
-// SwiGLU, whose product doubles the error.
-constexpr int kSumBlocks = 8, kSumBlocksAtOnce = 14, kMaxColumns32 = 128;
+// The tensor core cuts the sums it adds to: a sum of 7168 products came out 8e-6 off, of the 2-norm, where torch's 32-bit products are 1e-7 (few rows) to
+// 9e-7 off (600). For a result of 32 bits a sum in tensor memory therefore is of at most 512 of the inner length (4.5e-7 off), and the epilogue's
+// threads add the parts up in registers, which hold 128 columns. (896 at once, 8.6e-7 off, took 6.25 us for 16 rows of 7168 to 256 where this takes 6.45.)
+constexpr int kSumBlocks = 8, kMaxColumns32 = 128;
 constexpr int kManyStep = 32;  // columns of a source in the slabs come in so many where there are many
 constexpr int kCached = 4096;  // pairs whose experts a block keeps in shared memory
 
@@ -99,15 +98,6 @@ struct TilesParams {
     int* error;  // mapped host memory: where a wait that ran out is recorded
 };
 
-// a / b for a >= 0, b > 0. A block works out a dozen of them, one after the other, before its first copy is on its way: an integer division is
-// 100 cycles and more, this half of that. (The quotient of a + 1/2 is at least 1/(2 b) away from a whole number, and __fdividef
-// is off by 2^-22 of it.)
-__host__ __device__ __forceinline__ int quotient(int a, int b) {
-#ifdef __CUDA_ARCH__
-    if (a < 1 << 20) return (int)__fdividef((float)a + 0.5f, (float)b);
-#endif
-    return a / b;
-}
 __host__ __device__ __forceinline__ int parts_of(int n, int size) { return quotient(n + size - 1, size); }
 
 template <int kNumber>
@@ -352,7 +342,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     const int highest = whole_tiles > 0 ? height : rounds.part;
     const int weight_bytes = ((paired ? 2 : 1) * max(highest, kGrouped ? piece : 0) * kRowBytes + 1023) & ~1023, block_bytes = weight_bytes + wide * kRowBytes;
     const int blocks_all = parts_of(p.inner, kTileInner);
-    const int per_stage = min(blocks_all, max(1, quotient(kStageBytes + block_bytes / 2, block_bytes)));
+    const int per_stage = stage_blocks(blocks_all, block_bytes, kStageBytes, k32 ? kSumBlocks : blocks_all);
     const int stages = min(kMaxStages, quotient(kRingBytes, block_bytes * per_stage));
     // this block's part of the inner length, and its tiles
     const int split = kCut ? p.split : 1, part = kCut ? (int)blockIdx.x % split : 0;
@@ -412,8 +402,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
     };
     const bool spread = kOp == kLayerUp && !p.sorted;  // all tokens are a tile's columns
     const uint32_t stage_bytes = (uint32_t)per_stage * block_bytes;
-    // kDense32: of a sum in tensor memory, whole stages
-    const int sum_blocks = !paired && blocks <= kSumBlocksAtOnce ? blocks : max(1, kSumBlocks / per_stage) * per_stage;
+    const int sum_of = sum_blocks(per_stage, kSumBlocks);  // kDense32
     if (warp == 0) {
         if (elect_one()) {
             int stage = 0;
@@ -460,7 +449,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
                     if (!barrier_wait(sums_empty0 + 8 * buffer, ((n >> 1) & 1) ^ 1, &s.gave_up)) goto products_done;
                     tcgen05_after_sync();
                     bool add = false;
-                    const int end = k32 ? max(0, chunk - sum_blocks) : 0;
+                    const int end = k32 ? max(0, chunk - sum_of) : 0;
                     for (int left = chunk; left > end; left -= per_stage) {
                         uint64_t w = ring_descriptor + (stage * stage_bytes >> 4);
                         if (!barrier_wait(full0 + 8 * stage, phase, &s.gave_up)) goto products_done;
@@ -643,7 +632,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) product_tiles_kernel(const _
 #pragma unroll
                     for (int j = 0; j < 16; ++j) total[g][j] = 0.0f;
                 bool all = true;
-                for (int chunk = blocks; chunk > sum_blocks && all; chunk -= sum_blocks, ++n) {
+                for (int chunk = blocks; chunk > sum_of && all; chunk -= sum_of, ++n) {
                     all = named_all(1, kFinishers, barrier_wait(sums_full0 + 8 * (n & 1), (n >> 1) & 1, &s.gave_up));
                     if (!all) break;
                     tcgen05_after_sync();
