@@ -15,7 +15,7 @@ namespace {
 
 // A wait inside a kernel ends after this long whatever happens: every barrier here is completed by the same block (or its
 // cluster), so one that is not is a fault of this code, and it is to end in an error instead of a GPU that does not answer. Cycles: two
-// seconds at 2 GHz. (Not the global timer: reading it takes so long that a ring whose every wait did took 0.4 us a step, ten times
+// seconds at 2 GHz, from when the launch before is through. (Not the global timer: reading it takes so long that a ring whose every wait did took 0.4 us a step, ten times
 // what the step moved.)
 constexpr long long kWaitCycles = 4000000000ll;
 
@@ -176,11 +176,17 @@ __device__ __forceinline__ void barrier_arrive_there(uint32_t bar) {
 }
 // Waits for the phase of `parity`; false where the block has given up, or does now because the time has run out.
 __device__ __noinline__ bool barrier_wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    const long long begin = clock64();
+    long long begin = 0;
     for (;;) {
         for (int i = 0; i < 16; ++i)
             if (barrier_try(bar, parity)) return true;
         if (*gave_up) return false;
+        if (begin == 0) {
+            // A call's later launch may be here before the one in front of it is through, whose rows nothing here goes on without: that takes as
+            // long as it takes.
+            cudaGridDependencySynchronize();
+            begin = clock64();
+        }
         if (clock64() - begin > kWaitCycles) {
             *gave_up = 1;
             return false;
