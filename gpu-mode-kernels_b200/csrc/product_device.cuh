@@ -170,7 +170,10 @@ __device__ __forceinline__ uint32_t of_first_block(uint32_t bar) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(bar));
     return there;
 }
-// Says that sums have been read, and no more: a release would wait for all stores that this thread has on their way, 1.9 us with an SM full of them.
+// Says that sums have been read, and no more: a release would wait for all stores that this thread has on their way, 1.9 us with an SM full of them. Nothing
+// but tensor memory is handed over, and its order needs none: each thread's loads are through (tcgen05.wait::ld) before its
+// tcgen05.fence::before_thread_sync, after which the warp meets and one lane arrives; the products' thread has tcgen05.fence::after_thread_sync between its
+// wait and the next product. These two fences order tensor memory across any flag, a relaxed one too.
 __device__ __forceinline__ void barrier_arrive_there(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
